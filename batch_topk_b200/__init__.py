@@ -168,6 +168,70 @@ def logits_topk_status(d_workspace: int, M: int, V: int, D: int, k: int, stream:
     return rc
 
 
+ELEM_F16, ELEM_BF16, ELEM_F32 = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+MAX_EXPERTS = 1024
+MAX_EXPERTS_PER_TOKEN = 32
+
+
+def sample(d_logits: int, elem: int, rows: int, vocab: int, logits_stride: int, d_noise: int,
+           noise_stride: int, temperature: float, d_temperature: int, top_k: int, d_top_k: int,
+           top_p: float, d_top_p: int, min_p: float, d_min_p: int, d_tokens: int,
+           d_logprobs: int, stream: int = 0) -> int:
+    """bt_sample (no reference counterpart): one token for each row of logits, by temperature,
+    top-k, top-p and min-p, from given exponential noise; each d_ setting may be 0 (the number
+    beside it holds for the batch)."""
+    return _lib.load().bt_sample(d_logits, elem, rows, vocab, logits_stride, d_noise, noise_stride,
+                                 temperature, d_temperature, top_k, d_top_k, top_p, d_top_p, min_p,
+                                 d_min_p, d_tokens, d_logprobs, stream)
+
+
+def route(d_logits: int, elem: int, tokens: int, experts: int, stride: int, k: int, score: int,
+          d_bias: int, groups: int, topk_groups: int, renormalize: int, scale: float,
+          d_weights: int, d_experts: int, stream: int = 0) -> int:
+    """bt_route (no reference counterpart): the k experts of each token and their weights."""
+    return _lib.load().bt_route(d_logits, elem, tokens, experts, stride, k, score, d_bias, groups,
+                                topk_groups, renormalize, scale, d_weights, d_experts, stream)
+
+
+def route_backward(d_logits: int, elem: int, tokens: int, experts: int, stride: int, k: int,
+                   score: int, renormalize: int, scale: float, d_experts: int, d_grad: int,
+                   d_logits_grad: int, stream: int = 0) -> int:
+    """bt_route_backward (no reference counterpart): the weights' gradient to the logits."""
+    return _lib.load().bt_route_backward(d_logits, elem, tokens, experts, stride, k, score,
+                                         renormalize, scale, d_experts, d_grad, d_logits_grad,
+                                         stream)
+
+
+def expert_order(d_experts: int, n: int, experts: int, d_offsets: int, d_order: int,
+                 d_position: int, stream: int = 0) -> int:
+    """bt_expert_order (no reference counterpart): assignments sorted by expert, stable."""
+    return _lib.load().bt_expert_order(d_experts, n, experts, d_offsets, d_order, d_position,
+                                       stream)
+
+
+def dispatch(d_x: int, elem: int, tokens: int, k: int, width: int, stride: int, d_order: int,
+             d_rows: int, stream: int = 0) -> int:
+    """bt_dispatch (no reference counterpart): rows of tokens in the experts' order."""
+    return _lib.load().bt_dispatch(d_x, elem, tokens, k, width, stride, d_order, d_rows, stream)
+
+
+def combine(d_rows: int, elem: int, tokens: int, k: int, width: int, d_position: int,
+            d_weights: int, d_y: int, stream: int = 0) -> int:
+    """bt_combine (no reference counterpart): the weighted sum of each token's rows."""
+    return _lib.load().bt_combine(d_rows, elem, tokens, k, width, d_position, d_weights, d_y,
+                                  stream)
+
+
+def combine_backward(d_rows: int, d_grad: int, elem: int, tokens: int, k: int, width: int,
+                     grad_stride: int, d_position: int, d_live: int, d_weights: int,
+                     d_rows_grad: int, d_weights_grad: int, stream: int = 0) -> int:
+    """bt_combine_backward (no reference counterpart): combine's gradients."""
+    return _lib.load().bt_combine_backward(d_rows, d_grad, elem, tokens, k, width, grad_stride,
+                                           d_position, d_live, d_weights, d_rows_grad,
+                                           d_weights_grad, stream)
+
+
 def workspace_status(d_workspace: int, seg_num: int = 0, stream: int = 0):
     """Synchronously reads the device status of the last call on this workspace.
 

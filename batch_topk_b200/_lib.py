@@ -31,6 +31,13 @@ EXPORTED = (
     "bt_logits_topk_f16_workspace_size",
     "bt_logits_topk_f16",
     "bt_logits_topk_status",
+    "bt_sample",
+    "bt_route",
+    "bt_route_backward",
+    "bt_expert_order",
+    "bt_dispatch",
+    "bt_combine",
+    "bt_combine_backward",
     "bt_set_handoff_wait_tries",
     "bt_set_profile_events",
     "bt_device_info",
@@ -95,6 +102,25 @@ def load() -> C.CDLL:
         lib.bt_logits_topk_f16.restype = i32
         lib.bt_logits_topk_status.argtypes = [vp, i32, i32, i32, i32, vp]
         lib.bt_logits_topk_status.restype = i32
+        f32 = C.c_float
+        lib.bt_sample.argtypes = [vp, i32, i32, i32, i64, vp, i64, f32, vp, i32, vp, f32, vp, f32,
+                                  vp, vp, vp, vp]
+        lib.bt_sample.restype = i32
+        lib.bt_route.argtypes = [vp, i32, i32, i32, i64, i32, i32, vp, i32, i32, i32, f32, vp, vp,
+                                 vp]
+        lib.bt_route.restype = i32
+        lib.bt_route_backward.argtypes = [vp, i32, i32, i32, i64, i32, i32, i32, f32, vp, vp, vp,
+                                          vp]
+        lib.bt_route_backward.restype = i32
+        lib.bt_expert_order.argtypes = [vp, i32, i32, vp, vp, vp, vp]
+        lib.bt_expert_order.restype = i32
+        lib.bt_dispatch.argtypes = [vp, i32, i32, i32, i32, i64, vp, vp, vp]
+        lib.bt_dispatch.restype = i32
+        lib.bt_combine.argtypes = [vp, i32, i32, i32, i32, vp, vp, vp, vp]
+        lib.bt_combine.restype = i32
+        lib.bt_combine_backward.argtypes = [vp, vp, i32, i32, i32, i32, i64, vp, vp, vp, vp, vp,
+                                            vp]
+        lib.bt_combine_backward.restype = i32
         lib.bt_set_handoff_wait_tries.argtypes = [i32]
         lib.bt_set_handoff_wait_tries.restype = None
         lib.bt_set_profile_events.argtypes = [vp, vp]

@@ -15,12 +15,16 @@ REPO = os.path.dirname(HERE)
 SRC = os.path.join(HERE, "csrc", "batch_topk.cu")
 GEN_SRC = os.path.join(HERE, "csrc", "gen.cu")  # device-side input generation
 LOGITS_SRC = os.path.join(HERE, "csrc", "bt_logits.cu")  # logits producer, fused top-k epilogue
+SAMPLE_SRC = os.path.join(HERE, "csrc", "bt_sample.cu")  # sampling
+EXPERTS_SRC = os.path.join(HERE, "csrc", "bt_experts.cu")  # routing and experts' rows
 HEADERS = [os.path.join(HERE, "csrc", f) for f in ("bt_device.cuh", "bt_kernels.cuh", "bt_body.cuh",
                                                    "bt_elem.cuh", "bt_small.cuh",
-                                                   "bt_large.cuh", "bt_common.cuh", "bt_f32.cuh")] + [
+                                                   "bt_large.cuh", "bt_common.cuh", "bt_f32.cuh",
+                                                   "bt_values.cuh")] + [
     os.path.join(REPO, "include", "batch_topk_b200.h"),
     os.path.join(REPO, "include", "batch_topk_b200_gen.h"),
 ]
+SOURCES = [SRC, GEN_SRC, LOGITS_SRC, SAMPLE_SRC, EXPERTS_SRC]
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libbatch_topk_b200.so")
 
@@ -42,7 +46,7 @@ def up_to_date() -> bool:
     if not os.path.exists(LIB):
         return False
     t = os.path.getmtime(LIB)
-    return all(os.path.getmtime(p) <= t for p in [SRC, GEN_SRC, LOGITS_SRC, *HEADERS])
+    return all(os.path.getmtime(p) <= t for p in [*SOURCES, *HEADERS])
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -50,7 +54,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = LIB + ".tmp"
-    cmd = [nvcc(), *NVCC_FLAGS, "-o", tmp, SRC, GEN_SRC, LOGITS_SRC]
+    cmd = [nvcc(), *NVCC_FLAGS, "--threads", "0", "-o", tmp, *SOURCES]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
     res = subprocess.run(cmd, capture_output=True, text=True)

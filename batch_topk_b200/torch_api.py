@@ -3,6 +3,10 @@
     values, indices = topk(x, k)                      # x: [seg_num, seg_len] fp16/bf16/fp32 on CUDA
     values, indices = topk_segmented(x, offsets, k)   # x: 1-D fp16/bf16/fp32, offsets: int32 [seg_num+1]
 
+    tokens, logprobs = sample(logits, noise, ...)     # a token from each row of logits
+    weights, experts = route(logits, k, ...)          # experts of each token; with expert_order,
+                                                      # dispatch and combine (experts.py)
+
 Values come back in x's dtype (the input's own bit patterns), indices as int32, both
 [seg_num, k]; descending by value, lower index first among equal values, NaN last.
 """
@@ -27,6 +31,8 @@ from . import (
     batch_topk_half_workspace_size,
     workspace_status,
 )
+from .experts import ExpertOrder, combine, dispatch, expert_order, route  # noqa: F401
+from .sampling import sample  # noqa: F401
 
 # entry points per element type: (fixed, fixed workspace size, CSR, CSR workspace size)
 _ENTRY = {

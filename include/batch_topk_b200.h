@@ -174,6 +174,100 @@ int bt_logits_topk_f16(const void* d_hidden, const void* d_weight, int M, int V,
 
 int bt_logits_topk_status(const void* d_workspace, int M, int V, int D, int k, void* stream);
 
+/* Operators of a language model built on selection; no reference counterpart (the reference
+ * selects and stops, include/batch_topk.cuh:10-19).  Common to all of them: `elem` names the type
+ * of the values (BT_ELEM_*), strides count elements between rows (the values of a row are
+ * adjacent), pointers are aligned to their elements, a call is asynchronous on `stream` and needs
+ * no workspace, and cudaErrorInvalidValue answers a bad shape, a NULL or misaligned pointer or an
+ * unknown constant before anything is launched. */
+#define BT_ELEM_F16 0
+#define BT_ELEM_BF16 1
+#define BT_ELEM_F32 2
+
+/* One token for each row of logits [rows, vocab], by temperature, top-k, top-p and min-p, from
+ * given random numbers.  1 <= vocab <= BT_MAX_SEG_LEN.
+ *
+ * With m the row's largest logit and w_j = exp((x_j - m) / temperature), the kept tokens are those
+ * that pass every filter, in rank order (value descending, equal values by lower index):
+ *   top_k   the first top_k tokens (exactly that many, ties included); <= 0 or >= vocab: off;
+ *   top_p   tokens with less than top_p of the weight of the top_k tokens ranked before them, and
+ *           always the first; >= 1 or NaN: off;
+ *   min_p   tokens with w_j >= min(min_p, 1), that is, at least min_p of the best token's
+ *           probability; <= 0 or NaN: off.
+ * The token is the kept one with the largest w_j / noise_j, the lowest index among equals: with
+ * noise drawn from the exponential distribution with mean 1, token j comes with probability
+ * w_j / (sum of the kept w).  noise [rows, vocab] is float32 and positive (a quotient that is
+ * negative or NaN loses to all others).  temperature <= 0 or NaN: the best-ranked token.
+ *
+ * d_logprobs[r] is the token's log-probability under softmax(x / temperature) of the whole row,
+ * filters not applied (greedy rows: temperature 1).  NaN logits count as -inf, which is never
+ * kept; +inf logits share the whole probability.  A row of -inf and NaN alone gives token -1 and
+ * log-probability -inf.
+ *
+ * Each setting is one number for the batch, or, where its d_ pointer is not NULL, an array [rows]
+ * on the device (and the number is ignored). */
+int bt_sample(const void* d_logits, int elem, int rows, int vocab, long long logits_stride,
+              const float* d_noise, long long noise_stride, float temperature,
+              const float* d_temperature, int top_k, const int* d_top_k, float top_p,
+              const float* d_top_p, float min_p, const float* d_min_p, int* d_tokens,
+              float* d_logprobs, void* stream);
+
+#define BT_MAX_EXPERTS 1024
+#define BT_MAX_EXPERTS_PER_TOKEN 32
+#define BT_SCORE_SOFTMAX 0
+#define BT_SCORE_SIGMOID 1
+
+/* Routing: the k experts of each token and their weights, from logits [tokens, experts].
+ *
+ * Scores s are the softmax or the sigmoid of the logits.  Experts are chosen by the logits, or by
+ * s + d_bias (float32 [experts], not NULL; the bias balances the choice and takes no part in the
+ * weights).  groups > 1 cuts the experts into that many equal runs (groups <= 32 divides experts):
+ * a group's score is its best choice (softmax) or the sum of its two best s + bias (sigmoid), and
+ * only the topk_groups best groups stay (equal scores: the lower group).  The k best of what stays
+ * come in descending order, equal choices by lower index.  weights [tokens, k] (float32) are
+ * scale * s, or with renormalize scale * s / (sum of the chosen s + 1e-20).
+ *
+ * An expert whose logit is -inf or NaN, or whose s + bias is, is closed to the token.  When fewer
+ * than k are open, the remaining slots hold expert -1 and weight 0.
+ * k <= min(BT_MAX_EXPERTS_PER_TOKEN, experts / groups * topk_groups). */
+int bt_route(const void* d_logits, int elem, int tokens, int experts, long long stride, int k,
+             int score, const float* d_bias, int groups, int topk_groups, int renormalize,
+             float scale, float* d_weights, int* d_experts, void* stream);
+
+/* The gradient of bt_route's weights to the logits: d_grad [tokens, k] in, d_logits_grad
+ * [tokens, experts] out, in the logits' type.  d_experts is bt_route's output; the choice of
+ * experts, and so the bias, has no gradient. */
+int bt_route_backward(const void* d_logits, int elem, int tokens, int experts, long long stride,
+                      int k, int score, int renormalize, float scale, const int* d_experts,
+                      const float* d_grad, void* d_logits_grad, void* stream);
+
+/* The n assignments (expert numbers, e.g. bt_route's [tokens, k] read row by row) sorted by expert,
+ * equal experts in input order: expert e's are d_order[d_offsets[e] .. d_offsets[e + 1]), each an
+ * index into d_experts; d_position is the inverse.  Numbers outside [0, experts) are left out:
+ * their d_position is -1, and d_order ends with as many -1.  d_offsets holds experts + 1 values. */
+int bt_expert_order(const int* d_experts, int n, int experts, int* d_offsets, int* d_order,
+                    int* d_position, void* stream);
+
+/* Rows of x [tokens, width] in the experts' order: d_rows[p] = x[d_order[p] / k], and zeros where
+ * d_order[p] is -1 (or not below tokens * k).  d_rows is [tokens * k, width]. */
+int bt_dispatch(const void* d_x, int elem, int tokens, int k, int width, long long stride,
+                const int* d_order, void* d_rows, void* stream);
+
+/* y[t] = sum over j of d_weights[t, j] * d_rows[d_position[t, j]], in the order of j with float32
+ * sums, without the j whose position is -1 (or not below tokens * k).  d_weights NULL: weights of
+ * 1, which is bt_dispatch's gradient. */
+int bt_combine(const void* d_rows, int elem, int tokens, int k, int width, const int* d_position,
+               const float* d_weights, void* d_y, void* stream);
+
+/* bt_combine's gradients: d_rows_grad[p] = weight * grad of the token that row p belongs to (rows
+ * from *d_live on, which belong to none, are zero; d_live is d_offsets + experts), and
+ * d_weights_grad[t, j] = <grad[t], d_rows[d_position[t, j]]>.  Either output may be NULL;
+ * d_rows is read for d_weights_grad only. */
+int bt_combine_backward(const void* d_rows, const void* d_grad, int elem, int tokens, int k,
+                        int width, long long grad_stride, const int* d_position,
+                        const int* d_live, const float* d_weights, void* d_rows_grad,
+                        float* d_weights_grad, void* stream);
+
 /* Failure-path test hook (no reference counterpart): the number of tries each consumer <->
  * merger hand-off wait of the k <= 128 kernel makes before it gives up, for calls launched
  * after this one, process-wide.  0 makes those waits fail at once, so a call ends early with
