@@ -18,9 +18,8 @@ from typing import NamedTuple
 
 import torch
 
-from . import (BatchTopkError, MAX_EXPERTS, MAX_EXPERTS_PER_TOKEN, SCORE_SIGMOID, SCORE_SOFTMAX,
-               _lib)
-from .sampling import ELEM
+from . import MAX_EXPERTS, MAX_EXPERTS_PER_TOKEN, SCORE_SIGMOID, SCORE_SOFTMAX, _lib
+from .sampling import ELEM, launch
 
 SCORES = {"softmax": SCORE_SOFTMAX, "sigmoid": SCORE_SIGMOID}
 
@@ -37,13 +36,9 @@ class ExpertOrder(NamedTuple):
     position: torch.Tensor
 
 
-def _call(what, rc):
-    if rc != 0:
-        raise BatchTopkError(rc, what)
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _first_order(grad):
+    if grad.requires_grad:
+        raise RuntimeError("route, dispatch and combine have first-order gradients only")
 
 
 def _row_major(x):
@@ -62,11 +57,10 @@ def _route_forward(logits, k, score, bias, groups, topk_groups, renormalize, sca
     weights = torch.empty((tokens, k), dtype=torch.float32, device=dev)
     chosen = torch.empty((tokens, k), dtype=torch.int32, device=dev)
     if tokens:
-        with torch.cuda.device(dev):
-            _call("route", _lib.load().bt_route(
-                logits.data_ptr(), ELEM[logits.dtype], tokens, experts, logits.stride(0), k, score,
-                bias.data_ptr() if bias is not None else None, groups, topk_groups,
-                int(renormalize), scale, weights.data_ptr(), chosen.data_ptr(), _stream(dev)))
+        launch("route", _lib.load().bt_route, dev, logits.data_ptr(), ELEM[logits.dtype], tokens,
+               experts, logits.stride(0), k, score, None if bias is None else bias.data_ptr(),
+               groups, topk_groups, int(renormalize), scale, weights.data_ptr(),
+               chosen.data_ptr())
     return weights, chosen
 
 
@@ -78,11 +72,14 @@ class _Route(torch.autograd.Function):
         ctx.save_for_backward(logits, chosen)
         ctx.args = (k, score, renormalize, scale)
         ctx.mark_non_differentiable(chosen)
+        ctx.set_materialize_grads(False)
         return weights, chosen
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _):
+        if grad is None:
+            return (None,) * 8
+        _first_order(grad)
         logits, chosen = ctx.saved_tensors
         k, score, renormalize, scale = ctx.args
         tokens, experts = logits.shape
@@ -90,11 +87,9 @@ class _Route(torch.autograd.Function):
         out = torch.empty((tokens, experts), dtype=logits.dtype, device=dev)
         if tokens:
             grad = grad.float().contiguous()
-            with torch.cuda.device(dev):
-                _call("route backward", _lib.load().bt_route_backward(
-                    logits.data_ptr(), ELEM[logits.dtype], tokens, experts, logits.stride(0), k,
-                    score, int(renormalize), scale, chosen.data_ptr(), grad.data_ptr(),
-                    out.data_ptr(), _stream(dev)))
+            launch("route backward", _lib.load().bt_route_backward, dev, logits.data_ptr(),
+                   ELEM[logits.dtype], tokens, experts, logits.stride(0), k, score,
+                   int(renormalize), scale, chosen.data_ptr(), grad.data_ptr(), out.data_ptr())
         return out, None, None, None, None, None, None, None
 
 
@@ -153,10 +148,8 @@ def expert_order(experts: torch.Tensor, num_experts: int) -> ExpertOrder:
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
     order = torch.empty(n, dtype=torch.int32, device=dev)
     position = torch.empty_like(experts)
-    with torch.cuda.device(dev):
-        _call("expert_order", _lib.load().bt_expert_order(
-            experts.data_ptr(), n, num_experts, offsets.data_ptr(), order.data_ptr(),
-            position.data_ptr(), _stream(dev)))
+    launch("expert_order", _lib.load().bt_expert_order, dev, experts.data_ptr(), n, num_experts,
+           offsets.data_ptr(), order.data_ptr(), position.data_ptr())
     return ExpertOrder(offsets, order, position)
 
 
@@ -181,10 +174,8 @@ def _dispatch(x, order, k):
     dev = x.device
     rows = torch.empty((tokens * k, width), dtype=x.dtype, device=dev)
     if rows.numel():
-        with torch.cuda.device(dev):
-            _call("dispatch", _lib.load().bt_dispatch(
-                x.data_ptr(), ELEM[x.dtype], tokens, k, width, x.stride(0), order.data_ptr(),
-                rows.data_ptr(), _stream(dev)))
+        launch("dispatch", _lib.load().bt_dispatch, dev, x.data_ptr(), ELEM[x.dtype], tokens, k,
+               width, x.stride(0), order.data_ptr(), rows.data_ptr())
     return rows
 
 
@@ -194,10 +185,9 @@ def _combine(rows, position, weights):
     dev = rows.device
     y = torch.empty((tokens, width), dtype=rows.dtype, device=dev)
     if y.numel():
-        with torch.cuda.device(dev):
-            _call("combine", _lib.load().bt_combine(
-                rows.data_ptr(), ELEM[rows.dtype], tokens, k, width, position.data_ptr(),
-                weights.data_ptr() if weights is not None else None, y.data_ptr(), _stream(dev)))
+        launch("combine", _lib.load().bt_combine, dev, rows.data_ptr(), ELEM[rows.dtype], tokens, k,
+               width, position.data_ptr(), None if weights is None else weights.data_ptr(),
+               y.data_ptr())
     return y
 
 
@@ -208,8 +198,8 @@ class _Dispatch(torch.autograd.Function):
         return _dispatch(x, order, position.shape[1])
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _first_order(grad)
         position, = ctx.saved_tensors
         return _combine(grad.contiguous(), position, None), None, None
 
@@ -221,8 +211,8 @@ class _Combine(torch.autograd.Function):
         return _combine(rows, position, weights)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _first_order(grad)
         rows, weights, offsets, position = ctx.saved_tensors
         tokens, k = position.shape
         dev = rows.device
@@ -230,12 +220,12 @@ class _Combine(torch.autograd.Function):
         d_weights = torch.empty_like(weights) if ctx.needs_input_grad[1] else None
         if rows.numel():
             grad = _row_major(grad)
-            with torch.cuda.device(dev):
-                _call("combine backward", _lib.load().bt_combine_backward(
-                    rows.data_ptr(), grad.data_ptr(), ELEM[rows.dtype], tokens, k, rows.shape[1],
-                    grad.stride(0), position.data_ptr(), offsets[-1:].data_ptr(),
-                    weights.data_ptr(), d_rows.data_ptr() if d_rows is not None else None,
-                    d_weights.data_ptr() if d_weights is not None else None, _stream(dev)))
+            live = offsets.data_ptr() + 4 * (offsets.numel() - 1)
+            launch("combine backward", _lib.load().bt_combine_backward, dev, rows.data_ptr(),
+                   grad.data_ptr(), ELEM[rows.dtype], tokens, k, rows.shape[1], grad.stride(0),
+                   position.data_ptr(), live, weights.data_ptr(),
+                   None if d_rows is None else d_rows.data_ptr(),
+                   None if d_weights is None else d_weights.data_ptr())
         elif d_weights is not None:
             d_weights.zero_()
         return d_rows, d_weights, None, None

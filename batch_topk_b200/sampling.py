@@ -16,12 +16,20 @@ from . import BatchTopkError, ELEM_BF16, ELEM_F16, ELEM_F32, MAX_SEG_LEN, _lib
 ELEM = {torch.float16: ELEM_F16, torch.bfloat16: ELEM_BF16, torch.float32: ELEM_F32}
 
 
-def launch_stream(device, stream):
-    """The stream a call on `device` runs on: `stream`, or the device's current one."""
-    s = stream if stream is not None else torch.cuda.current_stream(device)
-    if s.device != device:
-        raise ValueError(f"stream is on {s.device}, the input on {device}")
-    return s
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream without its wrapper object
+
+
+def launch(what, entry, device, *args):
+    """entry(*args, stream) on `device` and its current stream.  The device guard and the stream
+    object cost microseconds, which small calls feel: neither is made when it is not needed."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = entry(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):  # the library launches on the current device
+            rc = entry(*args, _raw_stream(index))
+    if rc != 0:
+        raise BatchTopkError(rc, what)
 
 
 def _setting(name, value, rows, dtype, device, lo, hi):
@@ -66,29 +74,28 @@ def sample(logits: torch.Tensor, noise: torch.Tensor, *, temperature=1.0, top_k=
         if (tokens.dtype != torch.int32 or logprobs.dtype != torch.float32
                 or any(o.shape != (rows,) or o.device != dev or not o.is_contiguous() for o in out)):
             raise ValueError(f"out must be contiguous int32 and float32 tensors [{rows}] on {dev}")
-    with torch.cuda.device(dev):  # the library launches on the current device
-        s = launch_stream(dev, stream)
-        if s != torch.cuda.current_stream(dev):
-            for x in (logits, noise, d_t, d_k, d_p, d_mp):
-                if x is not None:
-                    x.record_stream(s)  # read on s: keep its memory from reuse until s has run
-        with torch.cuda.stream(s):
-            if logits.stride(1) != 1 and vocab > 1:
-                logits = logits.contiguous()
-            if noise.stride(1) != 1 and vocab > 1:
-                noise = noise.contiguous()
-            if out is None:
-                tokens = torch.empty(rows, dtype=torch.int32, device=dev)
-                logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
-            if rows == 0:
-                return tokens, logprobs
-            rc = _lib.load().bt_sample(
-                logits.data_ptr(), ELEM[logits.dtype], rows, vocab, logits.stride(0),
-                noise.data_ptr(), noise.stride(0), t, d_t.data_ptr() if d_t is not None else None,
-                k, d_k.data_ptr() if d_k is not None else None, p,
-                d_p.data_ptr() if d_p is not None else None, mp,
-                d_mp.data_ptr() if d_mp is not None else None, tokens.data_ptr(),
-                logprobs.data_ptr(), s.cuda_stream)
-    if rc != 0:
-        raise BatchTopkError(rc, "sample")
+    if stream is not None:
+        if stream.device != dev:
+            raise ValueError(f"stream is on {stream.device}, the input on {dev}")
+        for x in (logits, noise, d_t, d_k, d_p, d_mp):
+            if x is not None:
+                x.record_stream(stream)  # read there: keep its memory until the stream has run
+        with torch.cuda.stream(stream):
+            return sample(logits, noise, temperature=temperature, top_k=top_k, top_p=top_p,
+                          min_p=min_p, out=out)
+    if logits.stride(1) != 1 and vocab > 1:
+        logits = logits.contiguous()
+    if noise.stride(1) != 1 and vocab > 1:
+        noise = noise.contiguous()
+    if out is None:
+        tokens = torch.empty(rows, dtype=torch.int32, device=dev)
+        logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
+    if rows:
+        launch("sample", _lib.load().bt_sample, dev, logits.data_ptr(), ELEM[logits.dtype], rows,
+               vocab, logits.stride(0), noise.data_ptr(), noise.stride(0),
+               t, d_t if d_t is None else d_t.data_ptr(),
+               k, d_k if d_k is None else d_k.data_ptr(),
+               p, d_p if d_p is None else d_p.data_ptr(),
+               mp, d_mp if d_mp is None else d_mp.data_ptr(),
+               tokens.data_ptr(), logprobs.data_ptr())
     return tokens, logprobs

@@ -341,6 +341,15 @@ def test_whole_layer_on_another_stream():
 
 
 @pytest.mark.gpu
+def test_second_order_gradients_are_refused():
+    x = rand(4, 16, seed=1).requires_grad_()
+    weights, _ = api.route(x, 2)
+    g = rand(4, 2, seed=2).requires_grad_()
+    with pytest.raises(RuntimeError, match="first-order"):
+        torch.autograd.grad(weights, x, g, create_graph=True)
+
+
+@pytest.mark.gpu
 def test_refusals():
     x = rand(4, 16, seed=1)
     for args, kw in (((0,), {}), ((17,), {}), ((2,), dict(score="relu")),
