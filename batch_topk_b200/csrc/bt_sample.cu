@@ -8,18 +8,20 @@
 //
 // A block, or a cluster of blocks where there are few rows, takes a row:
 //   1. one pass over the row keeps the running maximum and sum of weights of each thread
-//      (rescaled when its maximum moves), and the maximum of every group of four 16-byte vectors
-//      a thread reads, in shared memory.  Without filters the race runs in this pass.
-//   2. a bound below which no kept element lies: for top-k the k-th largest group maximum (k
-//      groups have an element at or above it), for top-p alone the value whose weight times the
-//      vocabulary is the mass that top-p leaves out, for min-p its weight.  Only groups whose
+//      (rescaled when its maximum moves), and the maximum of every group of
+//      16-byte vectors a thread reads, in shared memory.  Without filters the race runs in this pass.
+//   2. a bound below which no kept element lies: for top-k the value that k group maxima reach
+//      (k groups have an element at or above it), for top-p alone the value whose weight times
+//      the vocabulary is the mass that top-p leaves out, for min-p its weight.  Only groups whose
 //      maximum reaches it are read again (from L2), and their elements at or above it become a
 //      list in shared memory, at most kCap long.
 //   3. the list is ranked (value descending, then index), weights are summed in that order, and
 //      the filters and the race are evaluated entry by entry.
-// A list that overflows is tightened by a histogram of the elements' log-weights (1/64 octave a
-// bin); a row that still overflows (flat rows: a nucleus of more than kCap tokens, top-k above
-// it, ties at the cut) is cut by bisecting the ordered values with whole passes over the row.
+// Where the list overflows (flat rows, a nucleus of thousands), a second pass counts and weighs all
+// elements in bins of their log-weight; the bin that holds the cut becomes the list, and the
+// third pass that gathers it also sums and races the elements above it.  What even this leaves
+// (thousands of equal values at the cut, +inf logits, top-p within a top-k of thousands) is cut
+// by bisecting the ordered values with whole passes.
 //
 // Every sum has an order fixed by the launch, or is over whole numbers: the same call gives the
 // same bits.
@@ -41,14 +43,16 @@ using u64 = unsigned long long;
 constexpr unsigned kAll = 0xFFFFFFFFu;
 constexpr float kNegInf = -INFINITY;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kBlocksPerSm = 4;
 constexpr int kGroup = 4;         // vectors a thread loads at a time
-constexpr int kMaxSlots = 32;     // group maxima a thread keeps
-constexpr int kCap = 2 * kThreads;  // list entries
-constexpr int kBins = 1024;       // log-weight histogram: 16 octaves of 64 bins
-constexpr float kBinsPerOctave = 64.0f;
+constexpr int kMaxSlots = 20;     // group maxima a thread keeps
+constexpr int kCap = 1024;        // list entries
+constexpr int kMaxHot = 2048;     // groups read again before threads go through their own
+constexpr int kBinsPerThread = 6;
+constexpr int kBins = kBinsPerThread * kThreads;  // log-weight histogram, see Sampler::bin
 
 struct Params {
   const void* logits;
@@ -82,6 +86,31 @@ __device__ __forceinline__ float exp2_approx(float v) {
   return r;
 }
 
+// Two float32 operations in one instruction.
+__device__ __forceinline__ u64 pack2(float a, float b) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(u64 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ u64 exp2_approx2(u64 v) {
+  float a, b;
+  unpack2(v, a, b);
+  return pack2(exp2_approx(a), exp2_approx(b));
+}
+
 // ---- a row's vectors ---------------------------------------------------------------------------
 
 // 16 bytes of a row as values, NaN read as -inf.
@@ -91,6 +120,7 @@ struct Vec;
 template <>
 struct Vec<Elem<float>> {
   static constexpr int kPer = 4;
+  static constexpr bool kBf16 = false;
   static __device__ __forceinline__ uint4 clean(uint4 r) {
     r.x = __float_as_uint(fmaxf(__uint_as_float(r.x), kNegInf));
     r.y = __float_as_uint(fmaxf(__uint_as_float(r.y), kNegInf));
@@ -104,9 +134,13 @@ struct Vec<Elem<float>> {
     x[2] = __uint_as_float(r.z);
     x[3] = __uint_as_float(r.w);
   }
-  static __device__ __forceinline__ float max(const uint4& r) {
-    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)),
-                 fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+  // Largest of two vectors' values, NaN ignored.
+  static __device__ __forceinline__ float max2(const uint4& r, const uint4& o) {
+    const float a = fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)),
+                          fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+    const float b = fmaxf(fmaxf(__uint_as_float(o.x), __uint_as_float(o.y)),
+                          fmaxf(__uint_as_float(o.z), __uint_as_float(o.w)));
+    return fmaxf(fmaxf(a, b), kNegInf);
   }
   static __device__ __forceinline__ uint4 neg_inf() {
     return make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);
@@ -127,6 +161,7 @@ __device__ __forceinline__ uint32_t as_word(T2 h) {
 template <class T2, uint32_t kInf2>
 struct Vec16 {
   static constexpr int kPer = 8;
+  static constexpr bool kBf16 = kInf2 == 0xFF80FF80u;
   static __device__ __forceinline__ uint32_t clean2(uint32_t w) {
     return as_word(__hmax2(as2<T2>(w), as2<T2>(kInf2)));
   }
@@ -143,10 +178,11 @@ struct Vec16 {
       x[2 * i + 1] = f.y;
     }
   }
-  static __device__ __forceinline__ float max(const uint4& r) {
-    const T2 a = __hmax2(as2<T2>(r.x), as2<T2>(r.y)), b = __hmax2(as2<T2>(r.z), as2<T2>(r.w));
+  static __device__ __forceinline__ float max2(const uint4& r, const uint4& o) {
+    const T2 a = __hmax2(__hmax2(as2<T2>(r.x), as2<T2>(r.y)), __hmax2(as2<T2>(r.z), as2<T2>(r.w)));
+    const T2 b = __hmax2(__hmax2(as2<T2>(o.x), as2<T2>(o.y)), __hmax2(as2<T2>(o.z), as2<T2>(o.w)));
     const float2 f = two(as_word(__hmax2(a, b)));
-    return fmaxf(f.x, f.y);
+    return fmaxf(fmaxf(f.x, f.y), kNegInf);
   }
   static __device__ __forceinline__ uint4 neg_inf() {
     return make_uint4(kInf2, kInf2, kInf2, kInf2);
@@ -166,18 +202,22 @@ template <>
 struct Vec<Elem<__nv_bfloat16>> : Vec16<__nv_bfloat162, 0xFF80FF80u> {};
 
 // One block's slice [v0, v1) of a row's 16-byte vectors, which start at the boundary at or below
-// the row's first element; elements outside the row read as -inf.
+// the row's first element.  The row's first and last vectors may reach outside it: there elements
+// read as -inf.  [i0, i1) is the slice without those two.
 template <class E>
 struct Slice {
   using T = typename E::T;
   using V = Vec<E>;
   static constexpr int kPer = V::kPer;
   const uint4* base;
-  int shift, vocab, vecs, v0, v1;
+  int shift, vocab, vecs, v0, v1, i0, i1;
 
-  __device__ __forceinline__ uint4 load(int v) const {
-    uint4 r = V::clean(__ldg(base + v));
-    if (v == 0 || v == vecs - 1) {  // the vectors that may reach outside the row
+  __device__ __forceinline__ uint4 raw(int v) const {
+    return v < v1 ? __ldg(base + v) : V::neg_inf();
+  }
+  // Vector v of the slice from its bytes: nothing from outside the row.
+  __device__ __forceinline__ uint4 fix(int v, uint4 r) const {
+    if (v == 0 || v == vecs - 1) {
       T* e = reinterpret_cast<T*>(&r);
       const uint4 low = V::neg_inf();
       const T* inf = reinterpret_cast<const T*>(&low);
@@ -189,16 +229,35 @@ struct Slice {
     }
     return r;
   }
+  __device__ __forceinline__ uint4 load(int v) const { return V::clean(fix(v, raw(v))); }
 
-  // f(index, value) for every element of the slice
+  // f(index, value) for every element of the vectors of the slice whose maximum passes; four
+  // vectors in flight.
+  template <class P, class F>
+  __device__ __forceinline__ void each(P pass, F f) const {
+    for (int first = v0 + static_cast<int>(threadIdx.x); first < v1; first += kGroup * kThreads) {
+      uint4 r[kGroup];
+#pragma unroll
+      for (int u = 0; u < kGroup; ++u) r[u] = raw(first + u * kThreads);
+#pragma unroll 1
+      for (int u = 0; u < kGroup; ++u) {
+        const int v = first + u * kThreads;
+        const uint4 now = V::clean(fix(v, r[0]));
+        r[0] = r[1];
+        r[1] = r[2];
+        r[2] = r[3];
+        if (v < v1 && pass(V::max2(now, now))) {
+          float x[kPer];
+          V::unpack(now, x);
+#pragma unroll
+          for (int q = 0; q < kPer; ++q) f(v * kPer + q - shift, x[q]);
+        }
+      }
+    }
+  }
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-    for (int v = v0 + static_cast<int>(threadIdx.x); v < v1; v += kThreads) {
-      float x[kPer];
-      V::unpack(load(v), x);
-#pragma unroll
-      for (int q = 0; q < kPer; ++q) f(v * kPer + q - shift, x[q]);
-    }
+    each([](float) { return true; }, f);
   }
 };
 
@@ -210,20 +269,34 @@ struct Sum {
 };
 
 struct Shared {
-  u64 list[kCap];      // the row's candidates, in the first block of the cluster
-  u64 sorted[kCap];    // this block's candidates before they join the list; then the ranked list
-  uint32_t hist[kBins];
+  u64 list[kCap];        // the row's candidates, in the first block of the cluster
+  union {
+    struct {
+      u64 sorted[kCap];    // this block's candidates before they join the list; then the ranked list
+      float2 score[kCap];  // weight and noise of the ranked list
+    };
+    struct {
+      uint32_t bins[kBins], weights[kBins];
+    };
+  };
+  uint32_t runs[kThreads];  // kth_bin's counts
+  union {
+    uint16_t hot[kMaxHot];  // groups to read again: slot * kThreads + thread
+    uint32_t place[256];
+  };
   float2 warp_stat[kWarps];
   float2 block_stat[kMaxCluster];
-  uint32_t warp_count[2][kWarps];
+  float block_mass[kMaxCluster];
+  uint32_t warp_count[kWarps];
   float warp_mass[kWarps];
   Sum warp_sum[kWarps];
   Sum sum[2];
   u64 warp_best[kWarps];
   u64 best[2];
-  uint32_t count, total, base;
-  int bin;
-  uint32_t bin_count;
+  uint32_t count, total, base, hot_count;
+  int bin, bin_end;        // found by find_bin: the bins that may hold the target,
+  uint32_t above, inside;  // the elements before them, and in them
+  float heavier;           // the weight before them
 };
 
 // Every block reads all blocks' parts in rank order, so all of them hold the same bits and take
@@ -304,15 +377,6 @@ struct Team {
     parity ^= 1;
     return v;
   }
-
-  // Number of true predicates, or sum of small counts, in this block.
-  __device__ __forceinline__ uint32_t block_count(uint32_t n, int which) {
-    n = __reduce_add_sync(kAll, n);
-    if ((threadIdx.x & 31) == 0) sh.warp_count[which][threadIdx.x >> 5] = n;
-    __syncthreads();
-    const int lane = threadIdx.x & 31;
-    return __reduce_add_sync(kAll, lane < kWarps ? sh.warp_count[which][lane] : 0u);
-  }
 };
 
 // ---- the kernel ----------------------------------------------------------------------------------
@@ -322,6 +386,7 @@ struct Sampler {
   using S = Slice<E>;
   using V = typename S::V;
   static constexpr int kPer = S::kPer;
+  static constexpr bool kBf16 = sizeof(typename E::T) == 2 && V::kBf16;
 
   const Params& p;
   Team& team;
@@ -347,157 +412,281 @@ struct Sampler {
            (0xFFFFFFFFu - static_cast<uint32_t>(i));
   }
 
-  // Histogram bin of a value, never falling as the value falls.
+  // Bins of log-weight, in 64ths of an octave below the maximum: 256 of width 1, 256 of 2, 256 of
+  // 4 and so on, taken from the exponent and mantissa of 256 + distance.  A smaller value never
+  // has a smaller bin; kBins: its weight is 0 in float32 (more than 190 octaves down).
   __device__ __forceinline__ int bin(float x) const {
-    const float a = x == m ? 0.0f : (m - x) * (c * kBinsPerOctave);
-    return a < static_cast<float>(kBins) ? static_cast<int>(a) : kBins;
+    const float t = x == m ? 256.0f : fmaf(m - x, c * 64.0f, 256.0f);
+    return t < 16384.0f
+               ? static_cast<int>((__float_as_uint(t) - __float_as_uint(256.0f)) >> 15)
+               : kBins;
+  }
+  // Bins [fine_of, fine_end] that hold too much are binned again, linearly in the value from their
+  // upper edge; elements of the bins before them are in fine bin -1, those after them in kBins.
+  int fine_of = -1, fine_end = -1;
+  float fine_top, fine_scale;
+  __device__ __forceinline__ void refine(int b, int end) {
+    fine_of = b;
+    fine_end = end;
+    fine_top = m - bin_start(b) * (1.0f / 64.0f) / c;
+    fine_scale = static_cast<float>(kBins) * 64.0f * c / (bin_start(end + 1) - bin_start(b));
+  }
+  __device__ __forceinline__ int fine_bin(float x) const {
+    const int b = bin(x);
+    if (fine_of < 0 || b >= kBins) return b;
+    if (b < fine_of) return -1;
+    if (b > fine_end) return kBins;
+    return min(max(static_cast<int>((fine_top - x) * fine_scale), 0), kBins - 1);
   }
 
-  __device__ __forceinline__ int first_vec(int slot_at) const {
-    return s.v0 + slot_at * p.groups_per_slot * kGroup * kThreads + static_cast<int>(threadIdx.x);
+  // Distance, in 64ths of an octave, at which bin b begins.
+  static __device__ __forceinline__ float bin_start(int b) {
+    return __uint_as_float(__float_as_uint(256.0f) + (static_cast<uint32_t>(b) << 15)) - 256.0f;
   }
 
-  // f(index, value) for every element of the groups whose maximum passes
-  template <class P, class F>
-  __device__ __forceinline__ void each_hot(P pass, F f) const {
+  // A value not above any value of bins up to b.
+  __device__ __forceinline__ float bin_floor(int b) const {
+    return m - (bin_start(b + 1) + 0.01f) * 1.000002f * (1.0f / 64.0f) / c -
+           fabsf(m) * 1e-6f;
+  }
+
+  __device__ __forceinline__ int first_vec(int slot_at, int thread) const {
+    return s.i0 + slot_at * p.groups_per_slot * kGroup * kThreads + thread;
+  }
+
+  // f(index, value, inside) for the elements of the groups whose maximum is at least `low`, called by
+  // whole warps: a lane takes one element of a group, and a warp keeps four groups' loads in
+  // flight.  Lanes without an element have `inside` false.
+  template <class F>
+  __device__ __forceinline__ void each_hot(float low, F f) {
+    constexpr int kAhead = 4;
+    constexpr int kGroupElems = kGroup * kPer;
+    constexpr int kPerWarp = 32 / kGroupElems;  // groups a warp takes at a time
+    using T = typename E::T;
+    if (threadIdx.x == 0) sh.hot_count = 0;
+    __syncthreads();
     for (int at = 0; at < p.slots; ++at) {
-      if (!pass(slot[at * kThreads + threadIdx.x])) continue;
-      const int first = first_vec(at);
-      for (int u = 0; u < p.groups_per_slot * kGroup; ++u) {
-        const int v = first + u * kThreads;
-        if (v >= s.v1) break;
-        float x[kPer];
-        V::unpack(s.load(v), x);
+      if (slot[at * kThreads + threadIdx.x] >= low) {
+        const uint32_t n = atomicAdd(&sh.hot_count, 1u);
+        if (n < kMaxHot) sh.hot[n] = static_cast<uint16_t>(at * kThreads + threadIdx.x);
+      }
+    }
+    __syncthreads();
+    const bool many = sh.hot_count > kMaxHot;
+    const int groups = (many ? p.slots * kThreads : static_cast<int>(sh.hot_count));
+    // item: one group of a slot; after them the row's first and last vectors, which no slot holds
+    const int items = groups * p.groups_per_slot + 1;
+    const int lane = threadIdx.x & 31, sub = lane / kGroupElems, e = lane % kGroupElems;
+    const T* row = reinterpret_cast<const T*>(s.base);
+    const int start = static_cast<int>(threadIdx.x >> 5) * kPerWarp * kAhead;
+    for (int i0 = start; i0 < items; i0 += kWarps * kPerWarp * kAhead) {
+      T value[kAhead];
+      int index[kAhead];
 #pragma unroll
-        for (int q = 0; q < kPer; ++q) f(v * kPer + q - s.shift, x[q]);
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * kPerWarp + sub;
+        int v = -1;
+        if (i < items - 1) {
+          const int g = i / p.groups_per_slot;
+          const int h = many ? g : sh.hot[g];
+          v = first_vec(h / kThreads, h % kThreads) +
+              ((i % p.groups_per_slot) * kGroup + e / kPer) * kThreads;
+          if (v >= s.i1) v = -1;
+        } else if (i == items - 1 && e < 2 * kPer) {
+          v = e < kPer ? 0 : s.vecs - 1;
+          if (v < s.v0 || v >= s.v1 || (v == 0 && e >= kPer)) v = -1;
+        }
+        index[u] = v * kPer + e % kPer - s.shift;
+        if (v < 0 || index[u] >= s.vocab) index[u] = -1;
+        if (index[u] >= 0) value[u] = row[index[u] + s.shift];
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const bool in = index[u] >= 0;
+        f(index[u], in ? fmaxf(E::to_float(value[u]), kNegInf) : kNegInf, in);
       }
     }
   }
 
-  // Pass 1 with the filters still to come.
-  __device__ __forceinline__ void scan(float& mt, float& zt) {
-    mt = kNegInf;
-    float z0 = 0.0f, z1 = 0.0f;
-    for (int at = 0; at < p.slots; ++at) {
+  // Pass 1 with the filters still to come.  A thread's weights are 2^(x c - ref) with ref the rounded
+  // product of its maximum and c, so one fused multiply-add gives the exponent with one rounding;
+  // join() undoes the difference between ref and the product.  The next group's loads are in
+  // flight while one is summed.  A NaN, which the maxima ignore, makes the sum NaN.
+  struct Running {
+    float top = kNegInf, ref = kNegInf;
+    u64 sums = 0;  // two
+  };
+  static __device__ __forceinline__ void raise(Running& w, float most, float c) {
+    if (most > w.top) {
+      const float old = w.ref;
+      w.top = most;
+      w.ref = __fmul_rn(most, c);
+      const float f = exp2_approx(old - w.ref);
+      float a, b;
+      unpack2(w.sums, a, b);
+      w.sums = pack2(a * f, b * f);
+    }
+  }
+  static __device__ __forceinline__ void add(Running& w, const uint4& r, float c) {
+    const u64 cc = pack2(c, c), rr = pack2(-w.ref, -w.ref);
+    float x[kPer];
+    V::unpack(r, x);
+#pragma unroll
+    for (int q = 0; q < kPer; q += 2) {
+      w.sums = add2(w.sums, exp2_approx2(fma2(pack2(x[q], x[q + 1]), cc, rr)));
+    }
+  }
+
+  struct Stat {
+    float top, sum;
+  };
+  static __device__ __noinline__ Stat scan(const S s, float c, float* slot, int slots,
+                                           int groups_per_slot) {
+    Running w;
+    if (threadIdx.x < 2) {  // the row's first and last vectors
+      const int v = threadIdx.x == 0 ? 0 : s.vecs - 1;
+      if (v >= s.v0 && v < s.v1 && (threadIdx.x == 0 || v > 0)) {
+        const uint4 r = s.fix(v, __ldg(s.base + v));
+        raise(w, V::max2(r, r), c);
+        if (w.top > kNegInf) add(w, r, c);
+      }
+    }
+    const int stride = kGroup * kThreads;
+    int first = s.i0 + static_cast<int>(threadIdx.x);
+    uint4 r[kGroup];
+#pragma unroll
+    for (int u = 0; u < kGroup; ++u) {
+      r[u] = V::neg_inf();
+      if (first + u * kThreads < s.i1) r[u] = __ldg(s.base + first + u * kThreads);
+    }
+    int whole = (s.i1 - s.i0) / stride;  // groups that every thread has in full
+    for (int at = 0; at < slots; ++at) {
       float top = kNegInf;
-      for (int g = 0; g < p.groups_per_slot; ++g) {
-        const int first = first_vec(at) + g * kGroup * kThreads;
-        if (first >= s.v1) break;
-        uint4 r[kGroup];
+      for (int g = 0; g < groups_per_slot; ++g) {
+        uint4 now[kGroup];
+        if (--whole >= 0) {
 #pragma unroll
-        for (int u = 0; u < kGroup; ++u) {
-          const int v = first + u * kThreads;
-          r[u] = v < s.v1 ? s.load(v) : V::neg_inf();
-        }
-        float most = V::max(r[0]);
-#pragma unroll
-        for (int u = 1; u < kGroup; ++u) most = fmaxf(most, V::max(r[u]));
-        top = fmaxf(top, most);
-        if (most > mt) {
-          const float f = exp2_approx((mt - most) * c);
-          z0 *= f;
-          z1 *= f;
-          mt = most;
-        }
-        if (most > kNegInf) {
+          for (int u = 0; u < kGroup; ++u) now[u] = r[u];
+        } else {
 #pragma unroll
           for (int u = 0; u < kGroup; ++u) {
-            float x[kPer];
-            V::unpack(r[u], x);
-#pragma unroll
-            for (int q = 0; q < kPer; q += 2) {
-              z0 += exp2_approx((x[q] - mt) * c);
-              z1 += exp2_approx((x[q + 1] - mt) * c);
-            }
+            now[u] = first + u * kThreads < s.i1 ? r[u] : V::neg_inf();
           }
+        }
+        first += stride;
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) {
+          if (first + u * kThreads < s.i1) r[u] = __ldg(s.base + first + u * kThreads);
+        }
+        const float most = fmaxf(V::max2(now[0], now[1]), V::max2(now[2], now[3]));
+        top = fmaxf(top, most);
+        raise(w, most, c);
+        if (most > kNegInf) {
+#pragma unroll
+          for (int u = 0; u < kGroup; ++u) add(w, now[u], c);
         }
       }
       slot[at * kThreads + threadIdx.x] = top;
     }
-    zt = z0 + z1;
+    float a, b;
+    unpack2(w.sums, a, b);
+    return Stat{w.top, a + b};
   }
 
   // Pass 1 without filters: the race runs along.  Within a thread quotients are compared in the
   // approximate weights (relative to the thread's maximum), so two elements of one thread whose
   // quotients agree to about 2^-20 may change places; the threads' winners are compared exactly.
-  __device__ __forceinline__ void scan_race(float& mt, float& zt, float& wx, int& wi) {
-    constexpr int kPair = 2;
-    const bool wide = s.shift == 0 && reinterpret_cast<uintptr_t>(noise) % 16 == 0;
-    mt = kNegInf;
-    wi = -1;
-    wx = kNegInf;
-    float z0 = 0.0f, z1 = 0.0f, lead = 0.0f;
-    for (int first = s.v0 + static_cast<int>(threadIdx.x); first < s.v1; first += kPair * kThreads) {
-      uint4 r[kPair];
-      float q[kPair][kPer];
+  // kPer float32 values, read once: 16 or 32 bytes in one load.
+  static __device__ __forceinline__ void load_wide(const float* from, float (&q)[4]) {
+    asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(q[0]), "=f"(q[1]), "=f"(q[2]), "=f"(q[3])
+                 : "l"(from));
+  }
+  static __device__ __forceinline__ void load_wide(const float* from, float (&q)[8]) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(q[0]), "=f"(q[1]), "=f"(q[2]), "=f"(q[3]), "=f"(q[4]), "=f"(q[5]),
+                   "=f"(q[6]), "=f"(q[7])
+                 : "l"(from));
+  }
+  static __device__ __forceinline__ void load_noise(const S& s, const float* noise, int v, bool wide,
+                                                    float (&q)[kPer]) {
+    const int i = v * kPer - s.shift;
+    if (wide && v < s.v1 && i + kPer <= s.vocab) {
+      load_wide(noise + i, q);
+    } else {
 #pragma unroll
-      for (int u = 0; u < kPair; ++u) {
-        const int v = first + u * kThreads;
-        r[u] = v < s.v1 ? s.load(v) : V::neg_inf();
-        const int i = v * kPer - s.shift;
-        if (wide && i + kPer <= s.vocab && v < s.v1) {
-#pragma unroll
-          for (int h = 0; h < kPer; h += 4) {
-            const float4 f = __ldcs(reinterpret_cast<const float4*>(noise + i + h));
-            q[u][h] = f.x;
-            q[u][h + 1] = f.y;
-            q[u][h + 2] = f.z;
-            q[u][h + 3] = f.w;
-          }
-        } else {
-#pragma unroll
-          for (int h = 0; h < kPer; ++h) {
-            const bool in = v < s.v1 && i + h >= 0 && i + h < s.vocab;
-            q[u][h] = in ? __ldg(noise + i + h) : 1.0f;
-          }
-        }
+      for (int h = 0; h < kPer; ++h) {
+        const bool in = v < s.v1 && i + h >= 0 && i + h < s.vocab;
+        q[h] = in ? __ldg(noise + i + h) : 1.0f;
       }
-      float most = V::max(r[0]);
+    }
+  }
+
+  struct Racer {
+    float top, sum, x;
+    int at;
+  };
+  static __device__ __noinline__ Racer scan_race(const S s, const float* noise, float c) {
+    const bool wide = s.shift == 0 && reinterpret_cast<uintptr_t>(noise) % (4 * kPer) == 0;
+    float mt = kNegInf, wx = kNegInf;
+    int wi = -1;
+    float ref = kNegInf, z0 = 0.0f, z1 = 0.0f, lead = 0.0f;
+    int v = s.v0 + static_cast<int>(threadIdx.x);
+    uint4 r = s.raw(v);
+    float next[kPer];
+    load_noise(s, noise, v, wide, next);
+    for (; v < s.v1; v += kThreads) {
+      const uint4 now = s.fix(v, r);
+      float q[kPer];
 #pragma unroll
-      for (int u = 1; u < kPair; ++u) most = fmaxf(most, V::max(r[u]));
+      for (int h = 0; h < kPer; ++h) q[h] = next[h];
+      r = s.raw(v + kThreads);
+      load_noise(s, noise, v + kThreads, wide, next);
+      const float most = V::max2(now, now);
       if (most > mt) {
-        const float f = exp2_approx((mt - most) * c);
+        const float old = ref;
+        mt = most;
+        ref = __fmul_rn(mt, c);
+        const float f = exp2_approx(old - ref);
         z0 *= f;
         z1 *= f;
         lead *= f;
-        mt = most;
       }
       if (most > kNegInf) {
+        float x[kPer];
+        V::unpack(now, x);
 #pragma unroll
-        for (int u = 0; u < kPair; ++u) {
-          float x[kPer];
-          V::unpack(r[u], x);
-#pragma unroll
-          for (int h = 0; h < kPer; ++h) {
-            const float w = exp2_approx((x[h] - mt) * c);
-            if (h & 1) z1 += w; else z0 += w;
-            if (w > lead * q[u][h] && q[u][h] >= 0.0f) {
-              lead = __fdividef(w, q[u][h]);
-              wx = x[h];
-              wi = (first + u * kThreads) * kPer + h - s.shift;
-            }
+        for (int h = 0; h < kPer; ++h) {
+          const float w = exp2_approx(fmaf(x[h], c, -ref));
+          if (h & 1) z1 += w; else z0 += w;
+          if (w > lead * q[h] && q[h] >= 0.0f) {
+            lead = __fdividef(w, q[h]);
+            wx = x[h];
+            wi = v * kPer + h - s.shift;
           }
         }
       }
     }
-    zt = z0 + z1;
+    return Racer{mt, z0 + z1, wx, wi};
   }
 
   // The row's maximum and sum of weights from the threads'.
   __device__ __forceinline__ void join(float mt, float zt) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto merge = [&](float a, float b, int width) {  // over groups of `width` lanes
-      float top = a;
+    auto moved = [&](float2 a, float top) {  // a's sum, with the larger maximum's reference
+      return a.x == top ? a.y : a.y * exp2_approx(__fmul_rn(a.x, c) - __fmul_rn(top, c));
+    };
+    auto merge = [&](float2 a, int width) {  // over groups of `width` lanes
+      float top = a.x;
       for (int o = width / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
-      float sum = a == top ? b : b * exp2_approx((a - top) * c);
+      float sum = moved(a, top);
       for (int o = width / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
       return make_float2(top, sum);
     };
-    float2 w = merge(mt, zt, 32);
+    float2 w = merge(make_float2(mt, zt), 32);
     if (lane == 0) sh.warp_stat[warp] = w;
     __syncthreads();
-    w = sh.warp_stat[lane & (kWarps - 1)];
-    w = merge(w.x, w.y, kWarps);
+    w = merge(sh.warp_stat[lane & (kWarps - 1)], kWarps);
     if (team.blocks > 1) {
       if (threadIdx.x < static_cast<unsigned>(team.blocks)) {
         *team.of(&sh.block_stat[team.rank], threadIdx.x) = w;
@@ -505,99 +694,265 @@ struct Sampler {
       team.cluster.sync();
       w = make_float2(kNegInf, 0.0f);
       for (int b = 0; b < team.blocks; ++b) w.x = fmaxf(w.x, sh.block_stat[b].x);
-      for (int b = 0; b < team.blocks; ++b) {
-        const float2 o = sh.block_stat[b];
-        w.y += o.x == w.x ? o.y : o.y * exp2_approx((o.x - w.x) * c);
-      }
+      for (int b = 0; b < team.blocks; ++b) w.y += moved(sh.block_stat[b], w.x);
     }
     m = w.x;
-    z = w.y;
+    z = w.y * exp2_approx(-fmaf(m, c, -__fmul_rn(m, c)));
   }
 
-  // A value that at least k group maxima of this block reach, with not many more where the values
-  // allow it; -inf where fewer than k groups are open.
-  __device__ __forceinline__ float kth_bound(uint32_t k) {
-    auto reach = [&](float v, int which) {
-      uint32_t n = 0;
-      for (int at = 0; at < p.slots; ++at) n += slot[at * kThreads + threadIdx.x] >= v;
-      return team.block_count(n, which);
-    };
-    float lo = kNegInf, hi = m, step = 4.0f / inv;
-    for (int it = 0; it < 14; ++it) {
-      const float mid = lo == kNegInf ? m - step : 0.5f * (lo + hi);
-      step *= 2.0f;
-      if (!(mid < hi && mid > lo)) break;
-      const uint32_t n = reach(mid, it & 1);
-      if (n >= k) {
-        lo = mid;
-        if (n <= k + k / 4 + 16) break;
-      } else {
-        hi = mid;
+  __device__ __forceinline__ void clear_bins() {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+      sh.bins[i] = 0;
+      sh.weights[i] = 0;
+    }
+  }
+
+  // sh.bin and sh.bin_end: the first bins at which the running count of sh.bins reaches `want`
+  // (BY_COUNT: one bin), or the running weight of sh.weights reaches `low` and `high`; with the
+  // counts before and in them.  kBins where none does.  One weight unit is `unit` of the weight at
+  // its bin's start.
+  template <bool BY_COUNT>
+  __device__ __forceinline__ void find_bin(uint32_t want, float low, float high, float unit) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b0 = threadIdx.x * kBinsPerThread;
+    if (threadIdx.x == 0) sh.bin = sh.bin_end = kBins;
+    uint32_t n[kBinsPerThread], cn = 0;
+    float w[kBinsPerThread], cw = 0.0f;
+#pragma unroll
+    for (int h = 0; h < kBinsPerThread; ++h) {
+      n[h] = sh.bins[b0 + h];
+      cn += n[h];
+      if (!BY_COUNT) {
+        const int from = fine_of < 0 ? b0 + h : fine_of;
+        w[h] = n[h] ? sh.weights[b0 + h] * unit * exp2f(bin_start(from) * (-1.0f / 64.0f)) : 0.0f;
+        cw += w[h];
       }
     }
-    return lo;
+    const uint32_t own_n = cn;
+    const float own_w = cw;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t yn = __shfl_up_sync(kAll, cn, o);
+      if (lane >= o) cn += yn;
+      if (!BY_COUNT) {
+        const float yw = __shfl_up_sync(kAll, cw, o);
+        if (lane >= o) cw += yw;
+      }
+    }
+    if (lane == 31) {
+      sh.warp_count[warp] = cn;
+      sh.warp_mass[warp] = cw;
+    }
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) {
+      cn += sh.warp_count[i];
+      if (!BY_COUNT) cw += sh.warp_mass[i];
+    }
+    cn -= own_n;  // now the sums before this thread's bins
+    cw -= own_w;
+    int hit = kBins, end = kBins;
+    uint32_t above = 0, through = 0;
+    float heavier = 0.0f;
+#pragma unroll
+    for (int h = 0; h < kBinsPerThread; ++h) {
+      if (!BY_COUNT) cw += w[h];
+      if (hit == kBins && (BY_COUNT ? cn + n[h] >= want : (n[h] && cw >= low))) {
+        hit = b0 + h;
+        above = cn;
+        if (!BY_COUNT) heavier = cw - w[h];
+      }
+      cn += n[h];
+      if (end == kBins && (BY_COUNT ? cn >= want : (n[h] && cw >= high))) {
+        end = b0 + h;
+        through = cn;
+      }
+    }
+    if (hit < kBins) atomicMin(&sh.bin, hit);
+    if (end < kBins) atomicMin(&sh.bin_end, end);
+    __syncthreads();
+    if (hit < kBins && sh.bin == hit) {
+      sh.above = above;
+      sh.heavier = heavier;
+    }
+    if (end < kBins && sh.bin_end == end) sh.inside = through;
+    __syncthreads();
+    if (threadIdx.x == 0) sh.inside -= sh.above;
+    __syncthreads();
   }
 
-  // Gathers the elements that pass into the first block's list; their number in the row.
-  template <class P>
-  __device__ __forceinline__ uint32_t gather(P pass) {
+  // A bin that k of the row's threads, or groups, reach with their maxima: k elements lie in the bins
+  // up to it.  Counted in runs of kBinsPerThread bins, one a thread.  The threads' maxima are near
+  // enough while k is at most three quarters of them: about 1.4 k elements reach the bound then.
+  __device__ __forceinline__ int kth_bin(uint32_t k, float mt) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) sh.bin = kBins - 1;
+    if (4 * k <= 3u * kThreads * team.blocks) {
+      const int b = bin(mt);
+      if (b < kBins) atomicAdd(&sh.runs[b / kBinsPerThread], 1u);
+    } else {
+      for (int at = 0; at < p.slots; ++at) {
+        const int b = bin(slot[at * kThreads + threadIdx.x]);
+        if (b < kBins) atomicAdd(&sh.runs[b / kBinsPerThread], 1u);
+      }
+    }
+    team.sync();
+    uint32_t own = 0;
+    for (int b = 0; b < team.blocks; ++b) own += team.of(sh.runs, b)[threadIdx.x];
+    uint32_t n = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(kAll, n, o);
+      if (lane >= o) n += y;
+    }
+    if (lane == 31) sh.warp_count[warp] = n;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) n += sh.warp_count[i];
+    if (n >= k && n - own < k) sh.bin = (static_cast<int>(threadIdx.x) + 1) * kBinsPerThread - 1;
+    __syncthreads();
+    return sh.bin;
+  }
+
+  __device__ __forceinline__ void open_list() {
     if (threadIdx.x == 0) {
       sh.count = 0;
       sh.total = 0;
     }
     team.sync();
-    u64* mine = team.blocks > 1 ? sh.sorted : sh.list;
-    each_hot(pass, [&](int i, float x) {
-      if (pass(x) && x > kNegInf) {
-        const uint32_t at = atomicAdd(&sh.count, 1u);
-        if (at < kCap) {
-          mine[at] = (static_cast<u64>(~value_key(x)) << 32) | static_cast<uint32_t>(i);
-        }
-      }
-    });
+  }
+  // Adds the elements of a whole warp's lanes with `in`.
+  __device__ __forceinline__ void push(int i, float x, bool in) {
+    const unsigned who = __ballot_sync(kAll, in);
+    if (who == 0) return;
+    const int lane = threadIdx.x & 31, first = __ffs(who) - 1;
+    uint32_t at = 0;
+    if (lane == first) at = atomicAdd(&sh.count, static_cast<uint32_t>(__popc(who)));
+    at = __shfl_sync(kAll, at, first) + __popc(who & ((1u << lane) - 1u));
+    if (in && at < kCap) put(at, i, x);
+  }
+  __device__ __forceinline__ void put(uint32_t at, int i, float x) {
+    (team.blocks > 1 ? sh.sorted : sh.list)[at] =
+        (static_cast<u64>(~value_key(x)) << 32) | static_cast<uint32_t>(i);
+  }
+  // Joins the blocks' candidates in the first block's list; their number in the row, and the sum
+  // of all blocks' `part` (a thread's weight of candidates).
+  __device__ __forceinline__ uint32_t close_list(float part, float* mass) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(kAll, part, o);
+    if ((threadIdx.x & 31) == 0) sh.warp_mass[threadIdx.x >> 5] = part;
     __syncthreads();
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) sum += sh.warp_mass[i];
     const uint32_t n = sh.count;
+    *mass = sum;
     if (team.blocks == 1) return n;
     if (threadIdx.x == 0) sh.base = atomicAdd(team.of(&sh.total, 0), n);
+    if (threadIdx.x < static_cast<unsigned>(team.blocks)) {
+      *team.of(&sh.block_mass[team.rank], threadIdx.x) = sum;
+    }
     __syncthreads();
     u64* to = team.of(sh.list, 0);
     const uint32_t base = sh.base;
     for (uint32_t i = threadIdx.x; i < n && i < kCap && base + i < kCap; i += kThreads) {
-      to[base + i] = mine[i];
+      to[base + i] = sh.sorted[i];
     }
     team.cluster.sync();
+    sum = 0.0f;
+    for (int b = 0; b < team.blocks; ++b) sum += sh.block_mass[b];
+    *mass = sum;
     return *team.of(&sh.total, 0);
   }
 
-  // Ranks the list of n <= kCap entries into sh.sorted, best first.
-  __device__ __forceinline__ void rank_list(uint32_t n) {
+  // The elements of the bins up to `last`, from the groups that reach it.
+  __device__ __forceinline__ uint32_t gather(int last, float* mass) {
+    float part = 0.0f;
+    const float low = bin_floor(last);
+    each_hot(low, [&](int i, float x, bool in) {
+      in = in && x > kNegInf && bin(x) <= last;
+      push(i, x, in);
+      if (in) part += exp2_approx((x - m) * c);
+    });
+    return close_list(part, mass);
+  }
+
+  // Drops entries of the first block's list of n that the cut cannot reach, by bins as in weigh();
+  // the rest go to sh.sorted.
+  __device__ __forceinline__ uint32_t prune(uint32_t n, bool by_k, uint32_t above, float mass) {
+    clear_bins();
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) weigh_one(entry_value(sh.list[i]), 32768.0f);
+    __syncthreads();
+    // the rounding of the bins' weights is below 2e-5 of them
+    if (by_k) {
+      find_bin<true>(static_cast<uint32_t>(top_k) - above, 0.0f, 0.0f, 0.0f);
+    } else {
+      const float target = top_p * z * 1.0001f - mass;
+      find_bin<false>(0, target, target, 1.0f / 32768.0f);
+    }
+    const int last = sh.bin_end;
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+      const u64 e = sh.list[i];
+      if (bin(entry_value(e)) <= last) sh.sorted[atomicAdd(&sh.count, 1u)] = e;
+    }
+    __syncthreads();
+    return sh.count;
+  }
+
+  static __device__ __forceinline__ float entry_value(u64 e) {
+    return key_value(~static_cast<uint32_t>(e >> 32));
+  }
+  // One element's count and weight to its bin; `units` of them are the weight at the bin's start.
+  __device__ __forceinline__ void weigh_one(float x, float units) {
+    const int b = fine_bin(x);
+    if (b < 0 || b >= kBins) return;
+    const float past = x == m ? 0.0f : fmaf(m - x, c * 64.0f, 256.0f) -
+                                           (bin_start(fine_of < 0 ? b : fine_of) + 256.0f);
+    atomicAdd(&sh.bins[b], 1u);
+    atomicAdd(&sh.weights[b],
+              static_cast<uint32_t>(exp2_approx(past * (-1.0f / 64.0f)) * units + 0.5f));
+  }
+
+  // Ranks n <= kCap entries (of sh.list, or in place) into sh.sorted, best first, and sets
+  // sh.score to the entries' weights and noise.
+  __device__ __forceinline__ void rank_list(const u64* list, uint32_t n) {
     if (n <= 256) {  // each entry's place is the number of entries before it
       uint32_t width = 32;
       while (width < n) width *= 2;
       const uint32_t mine = threadIdx.x & (width - 1), part = threadIdx.x / width;
       const uint32_t parts = kThreads / width;
-      uint32_t* place = sh.hist;
-      if (threadIdx.x < width) place[threadIdx.x] = 0;
+      uint32_t* place = sh.place;
+      const u64 e = mine < n ? list[mine] : ~0ull;
+      float2 score = make_float2(0.0f, 1.0f);
+      if (part == 0) {
+        place[mine] = 0;
+        if (mine < n) {
+          score.y = __ldg(noise + static_cast<uint32_t>(e));
+          score.x = weight(entry_value(e));
+        }
+      }
       __syncthreads();
-      const u64 e = mine < n ? sh.list[mine] : ~0ull;
       uint32_t before = 0;
-      for (uint32_t j = part; j < n; j += parts) before += sh.list[j] < e;
+      for (uint32_t j = part; j < n; j += parts) before += list[j] < e;
       if (mine < n && before) atomicAdd(&place[mine], before);
       __syncthreads();
-      if (part == 0 && mine < n) sh.sorted[place[mine]] = e;
+      if (part == 0 && mine < n) {
+        sh.sorted[place[mine]] = e;
+        sh.score[place[mine]] = score;
+      }
       __syncthreads();
       return;
     }
     uint32_t width = 512;
     while (width < n) width *= 2;
     for (uint32_t i = threadIdx.x; i < width; i += kThreads) {
-      sh.sorted[i] = i < n ? sh.list[i] : ~0ull;
+      sh.sorted[i] = i < n ? list[i] : ~0ull;
     }
     __syncthreads();
     for (uint32_t size = 2; size <= width; size *= 2) {
       for (uint32_t d = size / 2; d > 0; d /= 2) {
-        if (threadIdx.x < width / 2) {
-          const uint32_t a = (threadIdx.x / d) * 2 * d + threadIdx.x % d;
+        for (uint32_t i = threadIdx.x; i < width / 2; i += kThreads) {
+          const uint32_t a = 2 * (i & ~(d - 1)) | (i & (d - 1));
           const u64 x = sh.sorted[a], y = sh.sorted[a + d];
           if ((x > y) == ((a & size) == 0)) {
             sh.sorted[a] = y;
@@ -607,128 +962,149 @@ struct Sampler {
         __syncthreads();
       }
     }
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+      const u64 e = sh.sorted[i];
+      sh.score[i] = make_float2(weight(entry_value(e)), __ldg(noise + static_cast<uint32_t>(e)));
+    }
+    __syncthreads();
   }
 
-  // The winner of the list of n entries; first block only.
-  __device__ __forceinline__ u64 finish(uint32_t n, bool by_k) {
-    rank_list(n);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t stay = by_k && static_cast<uint32_t>(top_k) < n ? top_k : n;
-    float x[2], w[2], q[2];
-    int at[2];
+  // The winner among the list of n entries that follow `above` elements of weight `mass` in rank
+  // order: the filters and the race, 32 entries of the ranked list at a time.  First block only;
+  // the answer is the first warp's.
+  __device__ __forceinline__ u64 finish(uint32_t n, bool by_k, uint32_t above, float mass) {
+    const u64* list = sh.list;
+    if (n > 128) {
+      n = prune(n, by_k, above, mass);
+      list = sh.sorted;
+    }
+    rank_list(list, n);
+    if (threadIdx.x >= 32) return 0;
+    const uint32_t lane = threadIdx.x;
+    const uint32_t left = by_k ? static_cast<uint32_t>(top_k) - above : n;
+    const uint32_t stay = left < n ? left : n;
+    const bool by_p = top_p < 1.0f;
+    float target = top_p * z;
+    if (by_k && by_p) {
+      float all = 0.0f;
+      for (uint32_t i = lane; i < stay; i += 32) all += sh.score[i].x;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t i = threadIdx.x * 2 + h;
-      const u64 e = i < stay ? sh.sorted[i] : 0;
-      x[h] = i < stay ? key_value(~static_cast<uint32_t>(e >> 32)) : kNegInf;
-      at[h] = static_cast<int>(static_cast<uint32_t>(e));
-      q[h] = i < stay ? __ldg(noise + at[h]) : 1.0f;
-      w[h] = i < stay ? weight(x[h]) : 0.0f;
+      for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(kAll, all, o);
+      target = top_p * (mass + all);
     }
-    float run = w[0] + w[1];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float y = __shfl_up_sync(kAll, run, o);
-      if (lane >= o) run += y;
-    }
-    if (lane == 31) sh.warp_mass[warp] = run;
-    const float prev = __shfl_up_sync(kAll, run, 1);
-    __syncthreads();
-    float before = 0.0f, all = 0.0f;
-    for (int i = 0; i < kWarps; ++i) {
-      if (i < warp) before += sh.warp_mass[i];
-      all += sh.warp_mass[i];
-    }
-    if (lane > 0) before += prev;
-    const float target = top_p * (by_k ? all : z);
     u64 best = 0;
+    float before = mass;
+    for (uint32_t i = lane; i - lane < stay; i += 32) {
+      const float2 sc = i < stay ? sh.score[i] : make_float2(0.0f, 1.0f);
+      float run = sc.x;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t i = threadIdx.x * 2 + h;
-      const float ahead = h ? before + w[0] : before;
-      if (i < stay && (i == 0 || !(top_p < 1.0f) || ahead < target) && !(w[h] < min_p)) {
-        const float r = __fdiv_rn(w[h], q[h]);
+      for (int o = 1; o < 32; o <<= 1) {
+        const float y = __shfl_up_sync(kAll, run, o);
+        if (lane >= o) run += y;
+      }
+      const float prev = __shfl_up_sync(kAll, run, 1);
+      const float ahead = before + (lane ? prev : 0.0f);
+      const bool in = !by_p || ahead < target || i + above == 0;
+      if (i < stay && in && !(sc.x < min_p)) {
+        const float r = __fdiv_rn(sc.x, sc.y);
         const u64 e = (static_cast<u64>(value_key(r >= 0.0f ? r : -1.0f)) << 32) |
-                      (0xFFFFFFFFu - static_cast<uint32_t>(at[h]));
+                      (0xFFFFFFFFu - static_cast<uint32_t>(sh.sorted[i]));
         best = e > best ? e : best;
       }
+      before += __shfl_sync(kAll, run, 31);
+      if (by_p && !(before < target)) break;  // all later entries are out
     }
-    return team.block_best(best);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const u64 y = __shfl_xor_sync(kAll, best, o);
+      best = y > best ? y : best;
+    }
+    return best;
   }
 
-  // The last histogram bin that the wanted elements reach, and the number of elements up to it.
-  // Bins of whole counts: a count for top-k, and for top-p the least weight that a bin's elements
-  // can have.  kBins where that many octaves are not enough.
-  __device__ __forceinline__ int tighten(bool by_k, uint32_t* reach) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = 0;
+  // Pass 2 of an overflowing row: counts and weights by bin of the elements of the bins up to
+  // `last`, joined in every block; then sh.bin is the bin that holds the cut.
+  // `above` elements of weight `heavier` lie before the bins that are looked through.
+  __device__ __noinline__ void weigh(bool by_k, int last, uint32_t above, float heavier) {
+    const float units = fminf(32768.0f, 4.0e9f / static_cast<float>(p.vocab));
+    clear_bins();
     __syncthreads();
-    s.each([&](int, float x) {
-      const int b = bin(x);
-      if (b < kBins) atomicAdd(&sh.hist[b], 1u);
-    });
+    const float low = bin_floor(last);
+    s.each([&](float x) { return x >= low; },
+           [&](int, float x) {
+             if (x >= low && bin(x) <= last) weigh_one(x, units);
+           });
     team.sync();
-    if (team.blocks > 1) {
-      if (team.rank > 0) {
-        uint32_t* to = team.of(sh.hist, 0);
-        for (int i = threadIdx.x; i < kBins; i += kThreads) {
-          if (sh.hist[i]) atomicAdd(to + i, sh.hist[i]);
+    if (team.blocks > 1) {  // block b joins its share of the bins from all, and gives it to all
+      const int share = (kBins + team.blocks - 1) / team.blocks;
+      const int b0 = team.rank * share, b1 = min(b0 + share, kBins);
+      for (int i = b0 + static_cast<int>(threadIdx.x); i < b1; i += kThreads) {
+        uint32_t n = 0, w = 0;
+        for (int b = 0; b < team.blocks; ++b) {
+          n += team.of(sh.bins, b)[i];
+          w += team.of(sh.weights, b)[i];
+        }
+        for (int b = 0; b < team.blocks; ++b) {
+          team.of(sh.bins, b)[i] = n;
+          team.of(sh.weights, b)[i] = w;
         }
       }
       team.cluster.sync();
     }
-    if (team.rank == 0) {
-      if (threadIdx.x == 0) {
-        sh.bin = kBins;
-        sh.bin_count = 0;
-      }
-      __syncthreads();
-      const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-      uint32_t n[2];
-      float w[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int b = threadIdx.x * 2 + h;
-        n[h] = sh.hist[b];
-        w[h] = n[h] * exp2f(-(b + 1) / kBinsPerOctave) * 0.999f;
-      }
-      uint32_t cn = n[0] + n[1];
-      float cw = w[0] + w[1];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t yn = __shfl_up_sync(kAll, cn, o);
-        const float yw = __shfl_up_sync(kAll, cw, o);
-        if (lane >= o) {
-          cn += yn;
-          cw += yw;
+    if (by_k) {
+      find_bin<true>(static_cast<uint32_t>(top_k) - above, 0.0f, 0.0f, 0.0f);
+    } else {
+      const float slack = top_p * z * (0.6f / units + 2e-6f);  // the units' rounding
+      const float target = top_p * z - heavier;
+      find_bin<false>(0, target - slack, target + slack, 1.0f / units);
+    }
+  }
+
+  // Pass 3: the elements of the bins [at, end] into the list; those above them are all kept, so
+  // they are counted, summed and raced.  `inside`: the weight in the bins.
+  __device__ __noinline__ uint32_t split(int at, int end, Sum* above, double* inside, u64* best) {
+    open_list();
+    float za = 0.0f, zi = 0.0f;
+    uint32_t n = 0;
+    u64 top = 0;
+    const float low = bin_floor(fine_of < 0 ? end : fine_end);
+    s.each([&](float x) { return x >= low; }, [&](int i, float x) {
+      if (!(x >= low)) return;
+      const int b = fine_bin(x);
+      if (b > end) return;
+      const float w = weight(x);
+      if (b >= at) {
+        zi += w;
+        const uint32_t to = atomicAdd(&sh.count, 1u);
+        if (to < kCap) put(to, i, x);
+      } else {
+        za += w;
+        ++n;
+        if (!(w < min_p)) {
+          const u64 e = entry(x, i);
+          top = e > top ? e : top;
         }
       }
-      if (lane == 31) {
-        sh.warp_count[0][warp] = cn;
-        sh.warp_mass[warp] = cw;
-      }
-      __syncthreads();
-      for (int i = 0; i < warp; ++i) {
-        cn += sh.warp_count[0][i];
-        cw += sh.warp_mass[i];
-      }
-      const float target = top_p * z;
-      // inclusive sums at this thread's two bins
-      const uint32_t n1 = cn, n0 = cn - n[1];
-      const float w1 = cw, w0 = cw - w[1];
-      const bool hit0 = by_k ? n0 >= static_cast<uint32_t>(top_k) : w0 >= target;
-      const bool hit1 = by_k ? n1 >= static_cast<uint32_t>(top_k) : w1 >= target;
-      if (hit0 || hit1) atomicMin(&sh.bin, static_cast<int>(threadIdx.x) * 2 + (hit0 ? 0 : 1));
-      __syncthreads();
-      if (sh.bin / 2 == static_cast<int>(threadIdx.x)) sh.bin_count = (sh.bin & 1) ? n1 : n0;
-    }
-    team.sync();
-    const int b = *team.of(&sh.bin, 0);
-    *reach = *team.of(&sh.bin_count, 0);
-    return b;
+    });
+    float unused;
+    const uint32_t listed = close_list(0.0f, &unused);
+    *above = team.sum(za, n);
+    *inside = team.sum(zi, 0).mass;
+    *best = team.best(top);
+    return listed;
+  }
+
+  // Key k of the type's own values: float32 patterns of 16-bit types differ in their high bits only.
+  static constexpr int kKeyShift = sizeof(typename E::T) == 4 ? 0 : (kBf16 ? 16 : 13);
+  static __device__ __forceinline__ uint32_t short_key(float v) { return value_key(v) >> kKeyShift; }
+  static __device__ __forceinline__ float short_value(uint32_t k) {
+    const uint32_t low = (1u << kKeyShift) - 1u;
+    const uint32_t full = k << kKeyShift;
+    return key_value(full & 0x80000000u ? full : full | low);
   }
 
   // Whole passes: the cut in rank order by bisection, then the race over what is above it.
-  __device__ __forceinline__ u64 by_passes(double* total) {
+  __device__ __noinline__ u64 by_passes(float* total) {
     float zt = 0.0f;
     uint32_t n = 0;
     s.each([&](int, float x) {
@@ -738,22 +1114,22 @@ struct Sampler {
       }
     });
     const Sum all = team.sum(zt, n);
-    *total = all.mass;
+    *total = static_cast<float>(all.mass);
     // Elements above `cut` stay, and the first `ties` of those equal to it.
     float cut = kNegInf;
     uint32_t ties = 0;
     double mass_k = all.mass;
     if (top_k > 0 && static_cast<uint32_t>(top_k) < all.count) {
       // largest key with at least top_k elements at or above it
-      uint32_t lo = value_key(kNegInf), hi = value_key(m) + 1;
+      uint32_t lo = short_key(kNegInf), hi = short_key(m) + 1;
       while (hi - lo > 1) {
         const uint32_t mid = lo + (hi - lo) / 2;
-        const float v = key_value(mid);
+        const float v = short_value(mid);
         n = 0;
         s.each([&](int, float x) { n += x >= v; });
         if (team.sum(0.0f, n).count >= static_cast<uint32_t>(top_k)) lo = mid; else hi = mid;
       }
-      cut = key_value(lo);
+      cut = short_value(lo);
       float above = 0.0f;
       n = 0;
       s.each([&](int, float x) {
@@ -769,11 +1145,11 @@ struct Sampler {
     if (top_p < 1.0f) {
       const double target = static_cast<double>(top_p) * mass_k;
       // smallest key, not below the cut's, with less than the target above it
-      uint32_t lo = value_key(cut) - 1, hi = value_key(m);
+      uint32_t lo = short_key(cut) - 1, hi = short_key(m);
       double above_hi = 0.0;
       while (hi - lo > 1) {
         const uint32_t mid = lo + (hi - lo) / 2;
-        const float v = key_value(mid);
+        const float v = short_value(mid);
         float above = 0.0f;
         s.each([&](int, float x) { above += x > v ? weight(x) : 0.0f; });
         const Sum a = team.sum(above, 0);
@@ -784,7 +1160,7 @@ struct Sampler {
           lo = mid;
         }
       }
-      const float v = key_value(hi);
+      const float v = short_value(hi);
       // tie i (from 0) stays while the mass above it plus i weights is below the target
       const double stay = ceil((target - above_hi) / static_cast<double>(weight(v)));
       uint32_t few =
@@ -820,19 +1196,19 @@ struct Sampler {
     return team.best(best);
   }
 
-  __device__ __forceinline__ void write(u64 best, double total, long long r) const {
+  __device__ __forceinline__ void write(u64 best, float total, long long r) const {
     const int token = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(best));
     const float x = fmaxf(
         E::to_float(static_cast<const typename E::T*>(p.logits)[r * p.stride + token]), kNegInf);
     p.tokens[r] = token;
-    p.logprobs[r] = scaled(x) - static_cast<float>(log(total));
+    p.logprobs[r] = scaled(x) - logf(total);
   }
 };
 
 template <class E>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(Params p) {
-  __shared__ Shared sh;
-  extern __shared__ float slots[];
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(Params p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  Shared& sh = *reinterpret_cast<Shared*>(smem);
   Team team{cg::this_cluster(), sh, 1, 0};
   team.blocks = static_cast<int>(team.cluster.num_blocks());
   team.rank = static_cast<int>(team.cluster.block_rank());
@@ -840,7 +1216,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Params p) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(
       static_cast<const typename E::T*>(p.logits) + r * p.stride);
   Sampler<E> k{p, team, sh};
-  k.slot = slots;
+  k.slot = reinterpret_cast<float*>(smem + sizeof(Shared));
   k.noise = p.noise + r * p.noise_stride;
   k.s.base = reinterpret_cast<const uint4*>(at & ~static_cast<uintptr_t>(15));
   k.s.shift = static_cast<int>((at & 15) / sizeof(typename E::T));
@@ -849,6 +1225,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Params p) {
   const int per = (k.s.vecs + team.blocks - 1) / team.blocks;
   k.s.v0 = min(team.rank * per, k.s.vecs);
   k.s.v1 = min(k.s.v0 + per, k.s.vecs);
+  k.s.i0 = max(k.s.v0, 1);
+  k.s.i1 = min(k.s.v1, k.s.vecs - 1);
 
   const float t = p.d_temperature ? p.d_temperature[r] : p.temperature;
   k.top_k = p.d_top_k ? p.d_top_k[r] : p.top_k;
@@ -859,16 +1237,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Params p) {
   const bool by_k = k.top_k > 0 && k.top_k < p.vocab, by_p = k.top_p < 1.0f;
   const bool by_m = k.min_p > 0.0f;
   // T beyond these bounds makes all weights equal, or all but the largest 0, just as at them
-  k.inv = t > 0.0f ? fminf(fmaxf(__frcp_rn(t), 1e-37f), 1e38f) : 1.0f;
+  k.inv = t > 0.0f ? fminf(fmaxf(__frcp_rn(t), 1e-37f), 1e30f) : 1.0f;
   k.c = k.inv * kLog2e;
 
-  float mt, zt, wx;
-  int wi = -1;
   const bool open_race = !one && !by_k && !by_p && !by_m;
-  if (open_race) k.scan_race(mt, zt, wx, wi); else k.scan(mt, zt);
+  sh.runs[threadIdx.x] = 0;
+  if (threadIdx.x == 0) sh.count = sh.total = 0;  // an open list, seen by all after join()
+  float mt, zt, wx = 0.0f;
+  int wi = -1;
+  if (open_race) {
+    const auto out = Sampler<E>::scan_race(k.s, k.noise, k.c);
+    mt = out.top;
+    zt = out.sum;
+    wx = out.x;
+    wi = out.at;
+  } else {
+    const auto out = Sampler<E>::scan(k.s, k.c, k.slot, p.slots, p.groups_per_slot);
+    mt = out.top;
+    zt = out.sum;
+  }
   k.join(mt, zt);
-  u64 best = 0;
-  double total = k.z;
   if (k.m == kNegInf) {  // nothing open
     if (team.rank == 0 && threadIdx.x == 0) {
       p.tokens[r] = -1;
@@ -876,75 +1264,110 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Params p) {
     }
     return;
   }
-  bool passes = k.m == INFINITY;  // weights of +inf logits are equal: no approximate sums
-  if (!passes) {
-    if (one) {
-      k.each_hot([&](float x) { return x == k.m; },
-                 [&](int i, float x) {
-                   const u64 e = (1ull << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(i));
-                   if (x == k.m && e > best) best = e;
-                 });
-      best = team.best(best);
-    } else if (open_race) {
-      if (wi >= 0) best = k.entry(wx, wi);
-      best = team.best(best);
-      passes = (best >> 32) <= value_key(0.0f);  // every quotient 0 or none
-    } else if (!by_k && !by_p) {
-      // the approximate weight is within 2^-18 of the weight wherever it is above 2^-100
-      const float low = (k.min_p > 1e-30f ? log2f(k.min_p) : -100.0f) - 1e-4f;
-      k.each_hot([&](float x) { return (x - k.m) * k.c >= low || k.min_p <= 1e-30f; },
-                 [&](int i, float x) {
-                   if (x > kNegInf && !(k.weight(x) < k.min_p)) {
-                     const u64 e = k.entry(x, i);
-                     best = e > best ? e : best;
-                   }
-                 });
-      best = team.best(best);
-    } else {
-      float low = kNegInf;
-      if (by_k) {
-        low = k.kth_bound(static_cast<uint32_t>(k.top_k));
+  u64 best = 0;
+  float total = k.z;
+  // +inf or NaN logits (and products out of range): no approximate sums
+  bool passes = !(k.z < INFINITY) || k.m == INFINITY;
+  if (!passes && (by_k || by_p) && !one) {
+    // p alone starts from about 64 elements, which most rows' nuclei are within
+    const uint32_t want = by_k ? static_cast<uint32_t>(k.top_k) : 64u;
+    int last = min(k.kth_bin(want, mt), kBins - 1), lowest = last;
+    if (!by_k) {
+      // elements below weigh less than (1 - p) of the sum, were there a vocabulary of them
+      const float left = (1.0f - k.top_p) * k.z / static_cast<float>(p.vocab);
+      lowest = min(k.bin(k.m + (log2f(fmaxf(left, 1e-30f)) - 0.01f) / k.c), kBins - 1);
+      last = min(last, lowest);
+    }
+    uint32_t above = 0;
+    float mass, target = k.top_p * k.z * 1.0001f;
+    uint32_t n = k.gather(last, &mass);
+    u64 over = 0;
+    const bool few = !by_k && last < lowest && mass < target;
+    mass = 0.0f;
+    if (n > kCap || few) {
+      const int from = by_k ? last : lowest;
+      Sampler<E> slow = k;  // the rare functions stay out of line, and k in registers
+      slow.weigh(by_k, from, 0, 0.0f);
+      int at = sh.bin, end = sh.bin_end;
+      above = sh.above;
+      uint32_t inside = sh.inside;
+      if (end < kBins && inside > kCap && !(by_k && by_p)) {
+        const float heavier = sh.heavier;
+        __syncthreads();  // weigh() writes sh again
+        slow.refine(at, end);
+        slow.weigh(by_k, end, above, by_k ? 0.0f : heavier);
+        at = sh.bin;
+        end = sh.bin_end;
+        above += sh.above;
+        inside = sh.inside;
+      }
+      if (end < kBins && slow.fine_of < 0 && above + inside <= kCap) {
+        above = 0;
+        k.open_list();
+        float got;
+        n = k.gather(end, &got);
+        passes = n > kCap || (!by_k && end < lowest && got < k.top_p * k.z * 1.00001f);
+      } else if (end < kBins && inside <= kCap && !(by_k && by_p)) {
+        Sum up;
+        double in;
+        n = slow.split(at, end, &up, &in, &over);
+        mass = static_cast<float>(up.mass);
+        // the cut has to lie in these bins by the exact weights too
+        passes = by_p && !(mass < k.top_p * k.z && up.mass + in >= k.top_p * k.z);
       } else {
-        // elements below weigh less than (1 - p) of the sum, were there a vocabulary of them
-        const float left = (1.0f - k.top_p) * k.z / static_cast<float>(p.vocab);
-        low = k.m + (log2f(fmaxf(left, 1e-30f)) - 0.01f) / k.c;
-      }
-      uint32_t n = k.gather([&](float x) { return x >= low; });
-      if (n > kCap) {
-        uint32_t reach;
-        const int b = k.tighten(by_k, &reach);
-        if (b < kBins && reach <= kCap) {
-          n = k.gather([&](float x) { return k.bin(x) <= b; });
-        } else {
-          passes = true;
-        }
-      }
-      if (!passes) {
-        // the other blocks leave once every block has read the list's length
-        if (team.blocks > 1) team.cluster.barrier_arrive();
-        if (team.rank == 0) best = k.finish(n, by_k);
-        if (team.rank == 0 && threadIdx.x == 0) k.write(best, total, r);
-        if (team.blocks > 1) team.cluster.barrier_wait();
-        return;
+        passes = true;
       }
     }
-  }
-  if (passes) {
+    if (!passes) {
+      // the other blocks leave once every block has read the list's length
+      const bool alone = team.blocks == 1;
+      if (!alone) team.cluster.barrier_arrive();
+      if (team.rank == 0) {
+        best = k.finish(n, by_k, above, mass);
+        best = over > best ? over : best;
+        // every quotient 0 or none: an element of weight 0, beyond the list, may win
+        if (__syncthreads_or(threadIdx.x == 0 && (best >> 32) <= value_key(0.0f))) {
+          team.blocks = 1;
+          Sampler<E> slow = k;
+          slow.s.v0 = 0;
+          slow.s.v1 = slow.s.vecs;
+          best = slow.by_passes(&total);
+        }
+        if (threadIdx.x == 0) k.write(best, total, r);
+      }
+      if (!alone) team.cluster.barrier_wait();
+      return;
+    }
+  } else if (!passes) {
     if (one) {
-      k.top_k = 1;  // rank order alone decides
-      k.top_p = 1.0f;
-      k.min_p = 0.0f;
-      k.s.each([&](int i, float x) {
+      k.each_hot(k.m, [&](int i, float x, bool) {
         const u64 e = (1ull << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(i));
         if (x == k.m && e > best) best = e;
       });
-      best = team.best(best);
-      float zs = 0.0f;
-      k.s.each([&](int, float x) { zs += k.weight(x); });
-      total = team.sum(zs, 0).mass;
+    } else if (open_race) {
+      if (wi >= 0) best = k.entry(wx, wi);
     } else {
-      best = k.by_passes(&total);
+      // the exponent's rounding is far below 1e-4 wherever the weight is above 2^-100
+      const float low = k.min_p > 1e-30f ? k.m + (log2f(k.min_p) - 1e-4f) / k.c - fabsf(k.m) * 1e-6f
+                                         : kNegInf;
+      k.each_hot(low, [&](int i, float x, bool) {
+        if (x >= low && x > kNegInf && !(k.weight(x) < k.min_p)) {
+          const u64 e = k.entry(x, i);
+          best = e > best ? e : best;
+        }
+      });
     }
+    best = team.best(best);
+    passes = open_race && (best >> 32) <= value_key(0.0f);  // every quotient 0 or none
+  }
+  if (passes) {
+    Sampler<E> slow = k;
+    if (one) {  // rank order alone decides
+      slow.top_k = 1;
+      slow.top_p = 1.0f;
+      slow.min_p = 0.0f;
+    }
+    best = slow.by_passes(&total);
   }
   if (team.rank == 0 && threadIdx.x == 0) k.write(best, total, r);
   if (team.blocks > 1) team.cluster.sync();  // no block leaves while another may read its parts
@@ -958,10 +1381,10 @@ int launch(Params p, int blocks, cudaStream_t stream) {
   const long long groups = (per + kGroup * kThreads - 1) / (kGroup * kThreads);
   p.groups_per_slot = static_cast<int>((groups + kMaxSlots - 1) / kMaxSlots);
   p.slots = static_cast<int>((groups + p.groups_per_slot - 1) / p.groups_per_slot);
-  const int smem = p.slots * kThreads * static_cast<int>(sizeof(float));
-  cudaError_t e = cudaFuncSetAttribute(
-      sample_kernel<E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-      kMaxSlots * kThreads * static_cast<int>(sizeof(float)));
+  const int slot_bytes = kThreads * static_cast<int>(sizeof(float));
+  const int smem = static_cast<int>(sizeof(Shared)) + p.slots * slot_bytes;
+  cudaError_t e = cudaFuncSetAttribute(sample_kernel<E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(sizeof(Shared)) + kMaxSlots * slot_bytes);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * blocks);
@@ -981,10 +1404,10 @@ int launch(Params p, int blocks, cudaStream_t stream) {
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 // Blocks a row: as many as keep about two blocks on each of 148 SMs busy, but no more than leave
-// each thread a group of vectors.
+// each thread a vector.
 int blocks_for(int rows, int vocab, int per) {
   int blocks = 1;
-  while (blocks < kMaxCluster && static_cast<long long>(rows) * blocks < 2 * 148 &&
+  while (blocks < kMaxCluster && static_cast<long long>(rows) * blocks < 4 * 148 &&
          static_cast<long long>(vocab) > static_cast<long long>(blocks) * kThreads * per) {
     blocks *= 2;
   }
