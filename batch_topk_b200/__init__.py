@@ -172,6 +172,7 @@ ELEM_F16, ELEM_BF16, ELEM_F32 = 0, 1, 2
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 MAX_EXPERTS = 1024
 MAX_EXPERTS_PER_TOKEN = 32
+MAX_ASSIGNMENTS = 1 << 30
 
 
 def sample(d_logits: int, elem: int, rows: int, vocab: int, logits_stride: int, d_noise: int,
@@ -203,11 +204,15 @@ def route_backward(d_logits: int, elem: int, tokens: int, experts: int, stride: 
                                          stream)
 
 
+def expert_order_workspace_size(n: int, experts: int) -> int:
+    return int(_lib.load().bt_expert_order_workspace_size(n, experts))
+
+
 def expert_order(d_experts: int, n: int, experts: int, d_offsets: int, d_order: int,
-                 d_position: int, stream: int = 0) -> int:
+                 d_position: int, d_workspace: int, workspace_bytes: int, stream: int = 0) -> int:
     """bt_expert_order (no reference counterpart): assignments sorted by expert, stable."""
     return _lib.load().bt_expert_order(d_experts, n, experts, d_offsets, d_order, d_position,
-                                       stream)
+                                       d_workspace, workspace_bytes, stream)
 
 
 def dispatch(d_x: int, elem: int, tokens: int, k: int, width: int, stride: int, d_order: int,

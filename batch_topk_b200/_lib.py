@@ -35,6 +35,7 @@ EXPORTED = (
     "bt_route",
     "bt_route_backward",
     "bt_expert_order",
+    "bt_expert_order_workspace_size",
     "bt_dispatch",
     "bt_combine",
     "bt_combine_backward",
@@ -112,8 +113,10 @@ def load() -> C.CDLL:
         lib.bt_route_backward.argtypes = [vp, i32, i32, i32, i64, i32, i32, i32, f32, vp, vp, vp,
                                           vp]
         lib.bt_route_backward.restype = i32
-        lib.bt_expert_order.argtypes = [vp, i32, i32, vp, vp, vp, vp]
+        lib.bt_expert_order.argtypes = [vp, i32, i32, vp, vp, vp, vp, sz, vp]
         lib.bt_expert_order.restype = i32
+        lib.bt_expert_order_workspace_size.argtypes = [i32, i32]
+        lib.bt_expert_order_workspace_size.restype = sz
         lib.bt_dispatch.argtypes = [vp, i32, i32, i32, i32, i64, vp, vp, vp]
         lib.bt_dispatch.restype = i32
         lib.bt_combine.argtypes = [vp, i32, i32, i32, i32, vp, vp, vp, vp]

@@ -11,13 +11,12 @@
 // change from run to run.
 #include <cuda_runtime.h>
 
-#include <cooperative_groups.h>
 #include <cstdint>
+#include <mutex>
 
 #include "../../include/batch_topk_b200.h"
+#include "bt_device.cuh"
 #include "bt_values.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace bte {
 
@@ -25,12 +24,74 @@ using btv::Elem;
 
 constexpr unsigned kAll = 0xFFFFFFFFu;
 constexpr float kNegInf = -INFINITY;
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRenormEps = 1e-20f;  // keeps 0/0 away when every chosen score underflowed
+
+// VEC values that move as one word: loads and stores go through `raw`, values through value().
+template <int BYTES>
+struct Word;
+template <>
+struct Word<16> {
+  using type = uint4;
+};
+template <>
+struct Word<8> {
+  using type = uint2;
+};
+template <>
+struct Word<4> {
+  using type = uint32_t;
+};
+template <>
+struct Word<2> {
+  using type = uint16_t;
+};
+
+template <class E, int VEC>
+struct Pack {
+  using T = typename E::T;
+  using Raw = typename Word<sizeof(T) * VEC>::type;
+  Raw raw;
+  static __device__ __forceinline__ Pack load(const T* from) {
+    return Pack{*reinterpret_cast<const Raw*>(from)};
+  }
+  __device__ __forceinline__ void store(T* to) const { *reinterpret_cast<Raw*>(to) = raw; }
+  __device__ __forceinline__ float value(int q) const {
+    return E::to_float(reinterpret_cast<const T*>(&raw)[q]);
+  }
+  __device__ __forceinline__ void get(float (&x)[VEC]) const {
+    if constexpr (VEC % 2 == 0) {
+#pragma unroll
+      for (int q = 0; q < VEC; q += 2) E::to_floats(&raw, q, x[q], x[q + 1]);
+    } else {
+      x[0] = value(0);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&x)[VEC]) {
+    if constexpr (VEC % 2 == 0) {
+#pragma unroll
+      for (int q = 0; q < VEC; q += 2) E::from_floats(&raw, q, x[q], x[q + 1]);
+    } else {
+      *reinterpret_cast<T*>(&raw) = E::from_float(x[0]);
+    }
+  }
+};
+
+__device__ __forceinline__ float exp2_approx(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 
 // ---- routing ---------------------------------------------------------------------------------
 //
-// One warp a token; lane l owns the NPL experts from l * NPL, so a lower lane always holds
-// lower expert numbers and the first lane of a ballot resolves ties by index.
+// One warp a token; lane l owns the NPL experts from l * NPL, so a lower lane always holds lower
+// expert numbers and the first lane of a ballot resolves ties by index.
+//
+// The choice costs about one pass: the k-th largest of the lanes' maxima (a bitonic sort across
+// the warp) is a bound that at least k experts reach and few more (about 9 for k = 8 of 256).
+// Those go through shared memory to one lane each, and a lane's rank is the number of candidates
+// before its own.  More than 32 candidates (ties, or fewer than k open lanes) are taken one by one.
 
 struct RouteParams {
   const void* logits;
@@ -43,21 +104,16 @@ struct RouteParams {
   float scale;
 };
 
+constexpr int kRouteWarps = 4;
+
 // 1 / (1 + exp(-x)), each operation rounded once: the choice of experts compares these sums,
 // so no step may be contracted or approximated.
 __device__ __forceinline__ float sigmoid_rn(float x) {
   return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-x)));
 }
-
-// Order of the choice values as unsigned numbers, larger first; 0: closed (-inf or NaN).
-__device__ __forceinline__ uint32_t choice_key(float c) {
-  if (!(c > kNegInf)) return 0u;
-  const uint32_t b = __float_as_uint(__fadd_rn(c, 0.0f));  // -0 ranks as +0
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ float choice_value(uint32_t key) {
-  return key == 0 ? kNegInf
-                  : __uint_as_float((key & 0x80000000u) ? (key ^ 0x80000000u) : ~key);
+// The same within 1e-6, in four instructions.
+__device__ __forceinline__ float sigmoid_near(float x) {
+  return __fdividef(1.0f, 1.0f + exp2_approx(x * -kLog2e));
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -65,20 +121,46 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
   return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
+__device__ __forceinline__ float warp_max(float v) {  // no NaN
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Values of the warp sorted across its lanes, largest first.
+__device__ __forceinline__ float warp_sort_down(float v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
+  for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+    for (int d = size >> 1; d > 0; d >>= 1) {
+      const float o = __shfl_xor_sync(kAll, v, d);
+      v = ((lane & d) == 0) == ((lane & size) == 0) ? fmaxf(v, o) : fminf(v, o);
+    }
+  }
   return v;
 }
 
-// The lane's logits: NaN reads as -inf, and so does every place past the last expert.
-template <class E, int NPL>
+// The lane's logits: NaN reads as -inf, and so does every place past the last expert.  WIDE: the
+// rows are aligned for 16-byte loads and every lane's run is whole.
+template <class E, int NPL, bool WIDE>
 __device__ __forceinline__ void load_logits(const typename E::T* row, int num, float (&x)[NPL]) {
+  using T = typename E::T;
+  constexpr int kPer = 16 / sizeof(T) < NPL ? 16 / sizeof(T) : NPL;
   const int lane = threadIdx.x & 31;
+  if (WIDE) {
 #pragma unroll
-  for (int i = 0; i < NPL; ++i) {
-    const int e = lane * NPL + i;
-    x[i] = e < num ? fmaxf(E::to_float(row[e]), kNegInf) : kNegInf;
+    for (int i = 0; i < NPL; i += kPer) {
+      const auto v = Pack<E, kPer>::load(row + lane * NPL + i);
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) x[i + q] = fmaxf(v.value(q), kNegInf);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      const int e = lane * NPL + i;
+      x[i] = e < num ? fmaxf(E::to_float(row[e]), kNegInf) : kNegInf;
+    }
   }
 }
 
@@ -87,126 +169,228 @@ __device__ __forceinline__ float exp_below(float x, float m) {
   return m == kNegInf ? 0.0f : expf(x == m ? 0.0f : x - m);
 }
 
-// Softmax of the warp's row, with its maximum m and its sum of weights z.
 template <int NPL>
-__device__ __forceinline__ void softmax_row(const float (&x)[NPL], float (&s)[NPL], float& m,
-                                            float& z) {
-  m = kNegInf;
+__device__ __forceinline__ float row_max(const float (&x)[NPL]) {
+  float m = x[0];
 #pragma unroll
-  for (int i = 0; i < NPL; ++i) m = fmaxf(m, x[i]);
-  m = warp_max(m);
-  z = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NPL; ++i) {
-    s[i] = exp_below(x[i], m);
-    z += s[i];
-  }
-  z = fmaxf(warp_sum(z), 1e-30f);
-#pragma unroll
-  for (int i = 0; i < NPL; ++i) s[i] = __fdiv_rn(s[i], z);
+  for (int i = 1; i < NPL; ++i) m = fmaxf(m, x[i]);
+  return m;
 }
 
-template <class E, int NPL>
-__global__ void __launch_bounds__(128) route_kernel(RouteParams p) {
-  __shared__ uint32_t rows[4][32 * NPL];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long t = static_cast<long long>(blockIdx.x) * 4 + warp;
-  if (t >= p.tokens) return;
-  const auto* row = static_cast<const typename E::T*>(p.logits) + t * p.stride;
-  float x[NPL], s[NPL];
-  load_logits<E, NPL>(row, p.num, x);
-  if (p.sigmoid) {
+// exp(x - m) for finite m, approximately (2^-22).
+__device__ __forceinline__ float exp_near(float x, float m) {
+  return exp2_approx((x - m) * kLog2e);
+}
+
+// The sum of the row's weights exp(x - m), from approximate exponentials.  Rows of +inf logits count
+// them; a row with nothing open gives 1e-30.
+template <int NPL>
+__device__ __forceinline__ float row_sum(const float (&x)[NPL], float m) {
+  float z = 0.0f;
+  if (fabsf(m) < INFINITY) {
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) s[i] = sigmoid_rn(x[i]);
+    for (int i = 0; i < NPL; ++i) z += exp_near(x[i], m);
+    return warp_sum(z);
+  }
+  if (m == kNegInf) return 1e-30f;
+#pragma unroll
+  for (int i = 0; i < NPL; ++i) z += x[i] == m ? 1.0f : 0.0f;
+  return warp_sum(z);
+}
+
+// Before in the choice: the larger value, equal values by lower index (-0 equals +0).
+__device__ __forceinline__ bool before(float a, int ia, float b, int ib) {
+  return a > b || (a == b && ia < ib);
+}
+
+// The same order as a number, larger first: ordered bits of the choice, then the complement of the
+// expert's number.
+__device__ __forceinline__ unsigned long long place_key(float c, int e) {
+  const uint32_t b = __float_as_uint(__fadd_rn(c, 0.0f));
+  const uint32_t o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return (static_cast<unsigned long long>(o) << 32) | ~static_cast<uint32_t>(e);
+}
+__device__ __forceinline__ int place_expert(unsigned long long key) {
+  return static_cast<int>(~static_cast<uint32_t>(key));
+}
+
+// The groups' scores: sigmoid judges a group by its two best choices, softmax by its best.
+__device__ __forceinline__ void better_two(float& a, float& b, float oa, float ob) {
+  b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+  a = fmaxf(a, oa);
+}
+
+// Closes (sets to -inf) the choices of the groups that do not stay.
+template <int NPL>
+__device__ __forceinline__ void close_groups(const RouteParams& p, const float (&judged)[NPL],
+                                             float (&c)[NPL], float* shared) {
+  const int lane = threadIdx.x & 31, size = p.num / p.groups;
+  float a = kNegInf, b = kNegInf;  // this lane's group's two best, or of group `lane`
+  const int lanes = size / NPL;    // lanes a group covers, where it covers whole ones
+  const bool whole = lanes * NPL == size && (lanes & (lanes - 1)) == 0 && lanes > 0;
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) better_two(a, b, judged[i], kNegInf);
+    for (int o = 1; o < lanes; o <<= 1) {
+      const float oa = __shfl_xor_sync(kAll, a, o), ob = __shfl_xor_sync(kAll, b, o);
+      better_two(a, b, oa, ob);
+    }
   } else {
-    float m, z;
-    softmax_row<NPL>(x, s, m, z);
-  }
-  uint32_t key[NPL];
 #pragma unroll
-  for (int i = 0; i < NPL; ++i) {
-    const int e = lane * NPL + i;
-    const float b = (p.bias && e < p.num) ? p.bias[e] : 0.0f;
-    key[i] = x[i] == kNegInf ? 0u : choice_key(p.bias ? __fadd_rn(s[i], b) : x[i]);
-  }
-  if (p.groups > 1) {
-    // What a group is judged by: the choice, but the score where sigmoid has no bias (there
-    // the choice is the logit itself, which orders alike and does not saturate).
-    uint32_t* mine = rows[warp];
-#pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-      mine[lane * NPL + i] =
-          key[i] == 0 ? 0u : (p.sigmoid && !p.bias ? choice_key(s[i]) : key[i]);
+    for (int i = 0; i < NPL; ++i) shared[lane * NPL + i] = judged[i];
+    __syncwarp();
+    if (lane < p.groups) {
+      for (int i = 0; i < size; ++i) better_two(a, b, shared[lane * size + i], kNegInf);
     }
     __syncwarp();
-    const int size = p.num / p.groups;
-    uint32_t gkey = 0;
-    if (lane < p.groups) {
-      uint32_t a = 0, b = 0;  // the two best
-      for (int i = 0; i < size; ++i) {
-        const uint32_t v = mine[lane * size + i];
-        if (v > a) {
-          b = a;
-          a = v;
-        } else if (v > b) {
-          b = v;
-        }
-      }
-      gkey = a;
-      if (p.sigmoid && a) {
-        gkey = choice_key(__fadd_rn(choice_value(a), b ? choice_value(b) : 0.0f));
-      }
-    }
-    uint32_t stays = 0;
-    bool used = lane >= p.groups;
-    for (int r = 0; r < p.topk_groups; ++r) {
-      const uint32_t best = __reduce_max_sync(kAll, used ? 0u : gkey);
-      const unsigned at = __ballot_sync(kAll, !used && gkey == best);
-      const int g = __ffs(at) - 1;
-      stays |= 1u << g;
-      if (lane == g) used = true;
-    }
+  }
+  float score = a;
+  if (p.sigmoid && a > kNegInf) score = __fadd_rn(a, b > kNegInf ? b : 0.0f);
+  // rank of the lane's group among all
+  const int step = whole ? lanes : 1, mine = lane / step;
+  int rank = 0;
+  for (int g = 0; g < p.groups; ++g) {
+    const float o = __shfl_sync(kAll, score, g * step);
+    rank += before(o, g, score, mine);
+  }
+  const bool stays = mine < p.groups && rank < p.topk_groups;
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) c[i] = stays ? c[i] : kNegInf;
+  } else {
+    const unsigned kept = __ballot_sync(kAll, stays);
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
       const int e = lane * NPL + i;
-      if (e < p.num && !((stays >> (e / size)) & 1u)) key[i] = 0;
+      if (e < p.num && !((kept >> (e / size)) & 1u)) c[i] = kNegInf;
     }
   }
-  int my_expert = -1;
-  float my_score = 0.0f;
-  for (int j = 0; j < p.k; ++j) {
-    uint32_t best = 0;
+}
+
+template <class E, int NPL, bool WIDE>
+__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) {
+  __shared__ unsigned long long found[kRouteWarps][32];  // candidates, see place_key
+  __shared__ float rows[kRouteWarps][32 * NPL];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + warp;
+  if (t >= p.tokens) return;
+  const auto* row = static_cast<const typename E::T*>(p.logits) + t * p.stride;
+  float x[NPL];
+  load_logits<E, NPL, WIDE>(row, p.num, x);
+  float m = 0.0f, z = 1.0f;
+  if (!p.sigmoid) {
+    m = warp_max(row_max(x));
+    z = row_sum(x, m);
+  }
+  // the score of one logit
+  auto score_of = [&](float v) {
+    return p.sigmoid ? sigmoid_rn(v) : __fdiv_rn(exp_below(v, m), z);
+  };
+  // c: what is chosen by, -inf where the expert is closed
+  float c[NPL];
+  const bool grouped = p.groups > 1;
+  const bool near = p.bias && p.sigmoid && !grouped;  // c within 1e-6 first, exact for candidates
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) best = key[i] > best ? key[i] : best;
-    const uint32_t top = __reduce_max_sync(kAll, best);
-    if (top == 0) break;  // nothing open is left
-    const int from = __ffs(__ballot_sync(kAll, best == top)) - 1;
-    int at = -1;
-    float sc = 0.0f;
-#pragma unroll
-    for (int i = NPL - 1; i >= 0; --i) {
-      if (key[i] == top) {
-        at = i;
-        sc = s[i];
-      }
+  for (int i = 0; i < NPL; ++i) {
+    c[i] = x[i];
+    if (p.bias) {
+      const int e = lane * NPL + i;
+      const float b = e < p.num ? p.bias[e] : 0.0f;
+      const float s = near ? sigmoid_near(x[i]) : score_of(x[i]);
+      c[i] = x[i] == kNegInf ? kNegInf : fmaxf(__fadd_rn(s, b), kNegInf);
     }
-    if (lane == from) {
+  }
+  if (grouped) {
+    // sigmoid without bias: groups are judged by the scores, experts by the logits, which order
+    // alike and do not saturate
+    if (p.sigmoid && !p.bias) {
+      float s[NPL];
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) s[i] = x[i] == kNegInf ? kNegInf : sigmoid_rn(x[i]);
+      close_groups<NPL>(p, s, c, rows[warp]);
+    } else {
+      float judged[NPL];
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) judged[i] = c[i];
+      close_groups<NPL>(p, judged, c, rows[warp]);
+    }
+  }
+  // the bound, and who reaches it
+  const float sorted = warp_sort_down(row_max(c));
+  float bound = __shfl_sync(kAll, sorted, p.k - 1);
+  if (near) bound -= 4e-6f + 1e-6f * fabsf(bound);
+  bound = fmaxf(bound, -3.402823466e38f);  // closed experts are below every bound
+  int own = 0;
+#pragma unroll
+  for (int i = 0; i < NPL; ++i) own += c[i] >= bound;
+  int at = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(kAll, at, o);
+    if (lane >= o) at += y;
+  }
+  const int n = __shfl_sync(kAll, at, 31);
+  at -= own;
+  int expert = -1;  // slot `lane`
+  if (n <= 32) {
+    if (own) {
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
-        if (i == at) key[i] = 0;
+        if (c[i] >= bound) found[warp][at++] = place_key(c[i], lane * NPL + i);
       }
     }
-    const int e = __shfl_sync(kAll, lane * NPL + at, from);
-    sc = __shfl_sync(kAll, sc, from);
-    if (lane == j) {
-      my_expert = e;
-      my_score = sc;
+    __syncwarp();
+    unsigned long long mine = 0;
+    if (lane < n) {
+      mine = found[warp][lane];
+      if (near) {  // now exactly
+        const int e = place_expert(mine);
+        mine = place_key(
+            __fadd_rn(sigmoid_rn(fmaxf(E::to_float(row[e]), kNegInf)), p.bias[e]), e);
+      }
+    }
+    if (near) {
+      __syncwarp();
+      if (lane < n) found[warp][lane] = mine;
+      __syncwarp();
+    }
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += found[warp][j] > mine;
+    __syncwarp();
+    if (lane < n) found[warp][rank] = mine;
+    __syncwarp();
+    if (lane < (n < p.k ? n : p.k)) expert = place_expert(found[warp][lane]);
+  } else {
+    if (near) {
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        const int e = lane * NPL + i;
+        if (c[i] > kNegInf) c[i] = __fadd_rn(sigmoid_rn(x[i]), p.bias[e]);
+      }
+    }
+    for (int j = 0; j < p.k; ++j) {
+      const float best = row_max(c);
+      const float top = warp_max(best);
+      if (top == kNegInf) break;  // nothing open is left
+      const int from = __ffs(__ballot_sync(kAll, best == top)) - 1;
+      int at = 0;
+#pragma unroll
+      for (int i = NPL - 1; i >= 0; --i) at = c[i] == top ? i : at;
+      if (lane == from) {
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) c[i] = i == at ? kNegInf : c[i];
+      }
+      const int e = __shfl_sync(kAll, lane * NPL + at, from);
+      if (lane == j) expert = e;
     }
   }
-  const float total = p.renorm ? warp_sum(my_score) + kRenormEps : 1.0f;
+  const float score =
+      expert >= 0 ? score_of(fmaxf(E::to_float(row[expert]), kNegInf)) : 0.0f;
+  float weight = p.scale * score;
+  if (p.renorm) weight /= warp_sum(score) + kRenormEps;
   if (lane < p.k) {
-    p.weights[t * p.k + lane] = p.scale * my_score / total;
-    p.experts[t * p.k + lane] = my_expert;
+    p.weights[t * p.k + lane] = weight;
+    p.experts[t * p.k + lane] = expert;
   }
 }
 
@@ -226,27 +410,28 @@ struct RouteBackParams {
 //   sigmoid: dx_j = ds_j s_j (1 - s_j) at the chosen experts, 0 elsewhere;
 //   softmax: dx_i = s_i (ds_i - sum_j ds_j s_j) everywhere.
 // Each lane writes its own run first; the chosen experts' values then replace theirs.
-template <class E, int NPL>
-__global__ void __launch_bounds__(128) route_backward_kernel(RouteBackParams p) {
+template <class E, int NPL, bool WIDE>
+__global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(RouteBackParams p) {
+  using T = typename E::T;
+  constexpr int kPer = 16 / sizeof(T) < NPL ? 16 / sizeof(T) : NPL;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long t = static_cast<long long>(blockIdx.x) * 4 + warp;
+  const long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + warp;
   if (t >= p.tokens) return;
-  const auto* row = static_cast<const typename E::T*>(p.logits) + t * p.stride;
-  auto* out = static_cast<typename E::T*>(p.d_logits) + t * static_cast<long long>(p.num);
-  float x[NPL], s[NPL];
-  load_logits<E, NPL>(row, p.num, x);
+  const T* row = static_cast<const T*>(p.logits) + t * p.stride;
+  T* out = static_cast<T*>(p.d_logits) + t * static_cast<long long>(p.num);
   int e = lane < p.k ? p.experts[t * p.k + lane] : -1;
   if (e >= p.num) e = -1;
   const float g = e >= 0 ? p.scale * p.grad[t * p.k + lane] : 0.0f;
   const float xe = e >= 0 ? fmaxf(E::to_float(row[e]), kNegInf) : kNegInf;
-  float se, one_minus = 0.0f;
+  float x[NPL], m = 0.0f, z = 1.0f, se, one_minus = 0.0f;
   if (p.sigmoid) {
     const float u = expf(-fabsf(xe));
     se = sigmoid_rn(xe);
     one_minus = xe > 0.0f ? u / (1.0f + u) : 1.0f / (1.0f + u);
   } else {
-    float m, z;
-    softmax_row<NPL>(x, s, m, z);
+    load_logits<E, NPL, WIDE>(row, p.num, x);
+    m = warp_max(row_max(x));
+    z = row_sum(x, m);
     se = __fdiv_rn(exp_below(xe, m), z);
   }
   if (e < 0) se = 0.0f;
@@ -257,10 +442,34 @@ __global__ void __launch_bounds__(128) route_backward_kernel(RouteBackParams p) 
     ds = e >= 0 ? g / total - mean / total : 0.0f;
   }
   const float c = p.sigmoid ? 0.0f : warp_sum(ds * se);
+  float d[NPL];
+  if (p.sigmoid || m == kNegInf) {
 #pragma unroll
-  for (int i = 0; i < NPL; ++i) {
-    const int at = lane * NPL + i;
-    if (at < p.num) out[at] = E::from_float(p.sigmoid ? 0.0f : -s[i] * c);
+    for (int i = 0; i < NPL; ++i) d[i] = 0.0f;
+  } else if (m < INFINITY) {
+    const float f = -c / z;
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) d[i] = f * exp_near(x[i], m);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) d[i] = x[i] == m ? -c / z : 0.0f;
+  }
+  if (WIDE) {
+#pragma unroll
+    for (int i = 0; i < NPL; i += kPer) {
+      Pack<E, kPer> v;
+      float part[kPer];
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) part[q] = d[i + q];
+      v.set(part);
+      v.store(out + lane * NPL + i);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      const int at = lane * NPL + i;
+      if (at < p.num) out[at] = E::from_float(d[i]);
+    }
   }
   __syncwarp();
   if (e >= 0) out[e] = E::from_float(p.sigmoid ? ds * se * one_minus : se * (ds - c));
@@ -268,97 +477,231 @@ __global__ void __launch_bounds__(128) route_backward_kernel(RouteBackParams p) 
 
 // ---- order by expert ---------------------------------------------------------------------------
 //
-// Stable counting sort in one cluster.  The entries are cut into contiguous runs, one a warp, in
-// order over the cluster's blocks and warps; each warp counts its run's experts, the counts become
-// starting places (over experts, then blocks, then warps), and each warp places its run in order.
+// Stable counting sort.  The entries are cut into contiguous runs, one a block and, inside, one a
+// warp.  A first kernel counts each block's experts; the second sums those counts to the places
+// where its entries begin (over experts, then blocks, then warps), and ranks each warp's run 32
+// entries at a time: lanes with the same expert find each other by one ballot for each bit of its
+// number (the match instruction takes four times as long).  A block first places its entries in
+// shared memory, so that each expert's share leaves for memory in whole lines: single scattered
+// stores would cost a memory transaction for every entry.  Runs of more than kTile entries a block
+// go tile by tile, with the counts taken again for each tile.  Few entries take one block, which
+// counts for itself.
 
 struct OrderParams {
   const int* experts;
   int* offsets;
   int* order;
   int* position;
-  int n, num, per_warp;
+  uint32_t* counts;  // [blocks][num], where there is more than one block
+  int n, num;
+  int per_block;  // entries of a block, a multiple of 32 * kOrderWarps
 };
 
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
+constexpr int kTile = 32768;
+constexpr int kOrderAhead = 4;  // loads a lane keeps in flight
+constexpr int kOrderRun = 4096;  // entries of a block, more where that would take over kOrderBlocks
+constexpr int kOrderBlocks = 256;
 
-__global__ void __launch_bounds__(kOrderThreads) order_kernel(OrderParams p) {
+// Calls f(entry, expert, whether there is one) for the run [a0, a1), 32 entries at a time in order,
+// with every lane; the expert is -1 outside [0, num).
+template <class F>
+__device__ __forceinline__ void each_entry(const OrderParams& p, int a0, int a1, F f) {
+  const int lane = threadIdx.x & 31;
+  for (int a = a0; a < a1; a += 32 * kOrderAhead) {
+    int e[kOrderAhead];
+#pragma unroll
+    for (int u = 0; u < kOrderAhead; ++u) {
+      const int at = a + u * 32 + lane;
+      e[u] = at < a1 ? __ldg(p.experts + at) : -1;
+      if (static_cast<unsigned>(e[u]) >= static_cast<unsigned>(p.num)) e[u] = -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kOrderAhead; ++u) {
+      if (a + u * 32 < a1) f(a + u * 32 + lane, e[u], a + u * 32 + lane < a1);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kOrderThreads) order_count_kernel(OrderParams p) {
   extern __shared__ uint32_t smem[];
-  uint32_t* cnt = smem;                            // [warps][num]
-  uint32_t* tot = cnt + kOrderWarps * p.num;       // [num]: this block's counts
-  uint32_t* base = tot + p.num;                    // [num]: where this block's entries start
-  uint32_t* part = base + p.num;                   // [32]
-  cg::cluster_group cluster = cg::this_cluster();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned rank = cluster.block_rank(), blocks = cluster.num_blocks();
-  for (int i = threadIdx.x; i < kOrderWarps * p.num; i += kOrderThreads) cnt[i] = 0;
+  for (int e = threadIdx.x; e < p.num; e += kOrderThreads) smem[e] = 0;
   __syncthreads();
-  const long long first = (static_cast<long long>(rank) * kOrderWarps + warp) * p.per_warp;
-  const int a0 = static_cast<int>(first < p.n ? first : p.n);
-  const int a1 = static_cast<int>(first + p.per_warp < p.n ? first + p.per_warp : p.n);
-  uint32_t* mine = cnt + warp * p.num;
-  for (int a = a0 + lane; a < a1; a += 32) {
-    const int e = p.experts[a];
-    if (static_cast<unsigned>(e) < static_cast<unsigned>(p.num)) atomicAdd(&mine[e], 1u);
+  bt::grid_dep_launch();
+  const long long b0 = static_cast<long long>(blockIdx.x) * p.per_block;
+  const int last = static_cast<int>(b0 + p.per_block < p.n ? b0 + p.per_block : p.n);
+  for (int a = static_cast<int>(b0) + threadIdx.x; a < last; a += kOrderThreads * kOrderAhead) {
+    int e[kOrderAhead];
+#pragma unroll
+    for (int u = 0; u < kOrderAhead; ++u) {
+      const int at = a + u * kOrderThreads;
+      e[u] = at < last ? __ldg(p.experts + at) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kOrderAhead; ++u) {
+      if (static_cast<unsigned>(e[u]) < static_cast<unsigned>(p.num)) atomicAdd(&smem[e[u]], 1u);
+    }
   }
   __syncthreads();
   for (int e = threadIdx.x; e < p.num; e += kOrderThreads) {
-    uint32_t run = 0;
-    for (int w = 0; w < kOrderWarps; ++w) {
-      const uint32_t c = cnt[w * p.num + e];
-      cnt[w * p.num + e] = run;
-      run += c;
-    }
-    tot[e] = run;
+    p.counts[static_cast<size_t>(blockIdx.x) * p.num + e] = smem[e];
   }
-  cluster.sync();
-  // thread e: the cluster's count of expert e and the blocks' before this one (num <= threads)
-  uint32_t all = 0, before = 0;
-  if (threadIdx.x < p.num) {
-    for (unsigned b = 0; b < blocks; ++b) {
-      const uint32_t c = cluster.map_shared_rank(tot, b)[threadIdx.x];
-      all += c;
-      if (b < rank) before += c;
+}
+
+__global__ void __launch_bounds__(kOrderThreads) order_kernel(OrderParams p) {
+  extern __shared__ uint32_t smem[];
+  uint32_t* cnt = smem;                       // [warps][num]: counts, then starts in the tile
+  uint32_t* tot = cnt + kOrderWarps * p.num;  // [num]: the tile's counts
+  uint32_t* base = tot + p.num;               // [num]: where this block's next entries go
+  uint32_t* begin = base + p.num;             // [num]: where the tile's entries begin in `tile`
+  uint32_t* part = begin + p.num;             // [32]
+  uint16_t* tile = reinterpret_cast<uint16_t*>(part + 32);  // entries by expert
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank = blockIdx.x, blocks = gridDim.x;
+  const long long b0 = static_cast<long long>(rank) * p.per_block;
+  const int first = static_cast<int>(b0 < p.n ? b0 : p.n);
+  const int last = static_cast<int>(b0 + p.per_block < p.n ? b0 + p.per_block : p.n);
+  uint32_t* mine = cnt + warp * p.num;
+
+  auto clear = [&]() {
+    for (int i = threadIdx.x; i < kOrderWarps * p.num; i += kOrderThreads) cnt[i] = 0;
+    __syncthreads();
+  };
+  auto count = [&](int a0, int a1) {
+    each_entry(p, a0, a1, [&](int, int e, bool) {
+      if (e >= 0) atomicAdd(&mine[e], 1u);
+    });
+    __syncthreads();
+  };
+  // per-warp counts to starts within the expert; their sum to tot
+  auto starts = [&]() {
+    for (int e = threadIdx.x; e < p.num; e += kOrderThreads) {
+      uint32_t run = 0;
+      for (int w = 0; w < kOrderWarps; ++w) {
+        const uint32_t c = cnt[w * p.num + e];
+        cnt[w * p.num + e] = run;
+        run += c;
+      }
+      tot[e] = run;
     }
-  }
-  uint32_t incl = all;
+    __syncthreads();
+  };
+  // exclusive sum over the threads (num <= threads); total in *all
+  auto scan = [&](uint32_t v, uint32_t* all) {
+    uint32_t incl = v;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t y = __shfl_up_sync(kAll, incl, o);
-    if (lane >= o) incl += y;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(kAll, incl, o);
+      if (lane >= o) incl += y;
+    }
+    __syncthreads();
+    if (lane == 31) part[warp] = incl;
+    __syncthreads();
+    uint32_t w = part[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(kAll, w, o);
+      if (lane >= o) w += y;
+    }
+    *all = __shfl_sync(kAll, w, 31);
+    const uint32_t pre = __shfl_sync(kAll, w, warp ? warp - 1 : 0);
+    return (warp ? pre : 0u) + incl - v;
+  };
+  auto run_of = [&](int t0, int t1, int* a0, int* a1) {  // this warp's share of a tile
+    const int per = (t1 - t0 + 32 * kOrderWarps - 1) / (32 * kOrderWarps) * 32;
+    *a0 = min(t0 + warp * per, t1);
+    *a1 = min(*a0 + per, t1);
+  };
+
+  const int bits = 32 - __clz(p.num - 1 > 0 ? p.num - 1 : 1);  // of an expert's number
+  const bool one_tile = p.per_block <= kTile;
+  int a0, a1;
+  run_of(first, last, &a0, &a1);
+  clear();
+  count(a0, a1);
+  starts();
+  uint32_t all = 0, before = 0;  // thread e: the count of expert e, and earlier blocks'
+  if (blocks == 1) {
+    if (threadIdx.x < p.num) all = tot[threadIdx.x];
+  } else {
+    // the blocks' counts, summed by as many threads an expert as there are
+    bt::grid_dep_wait();
+    int width = 32;
+    while (width < p.num) width *= 2;
+    const int e = threadIdx.x & (width - 1), shares = kOrderThreads / width;
+    if (threadIdx.x < p.num) base[threadIdx.x] = begin[threadIdx.x] = 0;
+    __syncthreads();
+    if (e < p.num) {
+      uint32_t a = 0, b = 0;
+#pragma unroll 8
+      for (int i = threadIdx.x / width; i < blocks; i += shares) {
+        const uint32_t c = __ldcg(p.counts + static_cast<size_t>(i) * p.num + e);
+        a += c;
+        b += i < rank ? c : 0u;
+      }
+      atomicAdd(&base[e], a);  // base and begin hold the sums here
+      atomicAdd(&begin[e], b);
+    }
+    __syncthreads();
+    if (threadIdx.x < p.num) {
+      all = base[threadIdx.x];
+      before = begin[threadIdx.x];
+    }
+    __syncthreads();
   }
-  if (lane == 31) part[warp] = incl;
-  __syncthreads();
-  uint32_t pre = 0, live = 0;
-  for (int w = 0; w < kOrderWarps; ++w) {
-    if (w < warp) pre += part[w];
-    live += part[w];
-  }
+  uint32_t live;
+  const uint32_t at = scan(all, &live);
   if (threadIdx.x < p.num) {
-    base[threadIdx.x] = pre + incl - all + before;
-    if (rank == 0) p.offsets[threadIdx.x] = static_cast<int>(pre + incl - all);
+    base[threadIdx.x] = at + before;
+    if (rank == 0) p.offsets[threadIdx.x] = static_cast<int>(at);
   }
   if (rank == 0 && threadIdx.x == 0) p.offsets[p.num] = static_cast<int>(live);
-  __syncthreads();
-  for (int a = a0; a < a1; a += 32) {
-    const int at = a + lane;
-    int e = at < a1 ? p.experts[at] : -1;
-    if (static_cast<unsigned>(e) >= static_cast<unsigned>(p.num)) e = -1;
-    const unsigned peers = __match_any_sync(kAll, e);
-    const unsigned lower = peers & ((1u << lane) - 1u);
-    uint32_t start = 0;
-    if (e >= 0) start = mine[e];
-    __syncwarp();
-    if (e >= 0 && lower == 0) mine[e] = start + __popc(peers);
-    __syncwarp();
-    if (at < a1) {
-      int pos = -1;
-      if (e >= 0) {
-        pos = static_cast<int>(base[e] + start + __popc(lower));
-        p.order[pos] = at;
+
+  for (int t0 = first; t0 < last; t0 += kTile) {
+    const int t1 = min(t0 + kTile, last);
+    run_of(t0, t1, &a0, &a1);
+    if (!one_tile) {
+      __syncthreads();
+      clear();
+      count(a0, a1);
+      starts();
+    }
+    uint32_t in_tile;
+    const uint32_t from = scan(threadIdx.x < p.num ? tot[threadIdx.x] : 0u, &in_tile);
+    if (threadIdx.x < p.num) begin[threadIdx.x] = from;
+    __syncthreads();
+    each_entry(p, a0, a1, [&](int a, int e, bool in) {
+      unsigned peers = __ballot_sync(kAll, e >= 0);
+#pragma unroll
+      for (int b = 0; b < 10; ++b) {
+        if (b >= bits) break;
+        const bool set = (e >> b) & 1;
+        const unsigned who = __ballot_sync(kAll, set);
+        peers &= set ? who : ~who;
       }
-      p.position[at] = pos;
+      const unsigned lower = peers & ((1u << lane) - 1u);
+      uint32_t start = 0;
+      if (e >= 0) start = mine[e];
+      __syncwarp();
+      if (e >= 0 && lower == 0) mine[e] = start + __popc(peers);
+      __syncwarp();
+      if (in) {
+        int pos = -1;
+        if (e >= 0) {
+          const uint32_t r = start + __popc(lower);
+          pos = static_cast<int>(base[e] + r);
+          tile[begin[e] + r] = static_cast<uint16_t>(a - t0);
+        }
+        p.position[a] = pos;
+      }
+    });
+    __syncthreads();
+    for (int e = warp; e < p.num; e += kOrderWarps) {
+      const uint32_t n = tot[e], src = begin[e], dst = base[e];
+      for (uint32_t i = lane; i < n; i += 32) p.order[dst + i] = t0 + tile[src + i];
+      __syncwarp();
+      if (lane == 0) base[e] = dst + n;
     }
   }
   // places past the last live entry
@@ -366,113 +709,168 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(OrderParams p) {
        i += static_cast<long long>(blocks) * kOrderThreads) {
     p.order[i] = -1;
   }
-  cluster.sync();  // no block leaves while another may still read its counts
 }
 
 // ---- rows ----------------------------------------------------------------------------------------
 //
 // VEC elements a thread at a time: 16 bytes when the pointers, strides and width allow it, else one.
+// These kernels move bytes; what carries them is the number of independent loads in flight, so each
+// takes four rows at a time before the first is used.
+
+constexpr int kRowThreads = 256;
+constexpr int kAhead = 4;
 
 template <class E, int VEC>
-struct alignas(sizeof(typename E::T) * VEC) Pack {
-  typename E::T v[VEC];
-};
+__device__ __forceinline__ Pack<E, VEC> zero_pack() {
+  return Pack<E, VEC>{};
+}
 
+// Blocks take runs of rows, threads the vectors of a row; blockDim.y rows side by side where a row
+// is short.
 template <class E, int VEC>
-__global__ void dispatch_kernel(const typename E::T* x, long long stride, const int* order,
-                                typename E::T* rows, int tokens, int k, int nvec) {
+__global__ void __launch_bounds__(kRowThreads)
+    dispatch_kernel(const typename E::T* x, long long stride, const int* order,
+                    typename E::T* rows, int n, int k, int nvec) {
   using P = Pack<E, VEC>;
-  const long long total = static_cast<long long>(tokens) * k * nvec;
-  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const long long r = i / nvec;
-    const int c = static_cast<int>(i - r * nvec);
-    const int a = order[r];
-    P v;
-#pragma unroll
-    for (int q = 0; q < VEC; ++q) v.v[q] = E::from_float(0.0f);
-    if (a >= 0 && a < static_cast<long long>(tokens) * k) {
-      v = *reinterpret_cast<const P*>(x + (a / k) * stride + static_cast<long long>(c) * VEC);
+  const int side = blockDim.y, run = side * kAhead;  // a block's rows are neighbours
+  for (int r0 = blockIdx.x * run + threadIdx.y; r0 < n; r0 += gridDim.x * run) {
+    const typename E::T* from[kAhead];
+    // a lane looks up one row for its warp (whose threads all have the same threadIdx.y)
+    const int lane = threadIdx.x & 31;
+    long long start = -1;
+    if (lane < kAhead && r0 + lane * side < n) {
+      const int a = order[r0 + lane * side];
+      if (a >= 0 && a < n) start = (a / k) * stride;
     }
-    *reinterpret_cast<P*>(rows + (r * nvec + c) * VEC) = v;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const long long at = __shfl_sync(kAll, start, u);
+      from[u] = at >= 0 ? x + at : nullptr;
+    }
+    for (int c = threadIdx.x; c < nvec; c += blockDim.x) {
+      P v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        v[u] = from[u] ? P::load(from[u] + static_cast<long long>(c) * VEC) : zero_pack<E, VEC>();
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const long long r = r0 + u * side;
+        if (r < n) v[u].store(rows + (r * nvec + c) * VEC);
+      }
+    }
   }
 }
 
 template <class E, int VEC>
-__global__ void combine_kernel(const typename E::T* rows, const int* position,
-                               const float* weights, typename E::T* y, int tokens, int k,
-                               int nvec) {
+__global__ void __launch_bounds__(kRowThreads)
+    combine_kernel(const typename E::T* rows, const int* position, const float* weights,
+                   typename E::T* y, int tokens, int k, int nvec) {
   using P = Pack<E, VEC>;
-  const long long total = static_cast<long long>(tokens) * nvec;
   const long long n = static_cast<long long>(tokens) * k;
-  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const long long t = i / nvec;
-    const int c = static_cast<int>(i - t * nvec);
-    float acc[VEC];
+  for (int t = blockIdx.x * blockDim.y + threadIdx.y; t < tokens; t += gridDim.x * blockDim.y) {
+    const int* at = position + static_cast<long long>(t) * k;
+    const float* wt = weights ? weights + static_cast<long long>(t) * k : nullptr;
+    for (int c = threadIdx.x; c < nvec; c += blockDim.x) {
+      float acc[VEC];
 #pragma unroll
-    for (int q = 0; q < VEC; ++q) acc[q] = 0.0f;
-    for (int j = 0; j < k; ++j) {
-      const int at = position[t * k + j];
-      if (at < 0 || at >= n) continue;
-      const float w = weights ? weights[t * k + j] : 1.0f;
-      const P v = *reinterpret_cast<const P*>(rows + (static_cast<long long>(at) * nvec + c) * VEC);
+      for (int q = 0; q < VEC; ++q) acc[q] = 0.0f;
+      for (int j0 = 0; j0 < k; j0 += kAhead) {
+        P v[kAhead];
+        float w[kAhead];
 #pragma unroll
-      for (int q = 0; q < VEC; ++q) acc[q] = fmaf(w, E::to_float(v.v[q]), acc[q]);
+        for (int u = 0; u < kAhead; ++u) {
+          const int a = j0 + u < k ? at[j0 + u] : -1;
+          const bool in = a >= 0 && a < n;
+          w[u] = in && wt ? wt[j0 + u] : 1.0f;
+          v[u] = in ? P::load(rows + (static_cast<long long>(a) * nvec + c) * VEC)
+                    : zero_pack<E, VEC>();
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          if (j0 + u >= k) break;
+          float r[VEC];
+          v[u].get(r);
+#pragma unroll
+          for (int q = 0; q < VEC; ++q) acc[q] = fmaf(w[u], r[q], acc[q]);
+        }
+      }
+      P o;
+      o.set(acc);
+      o.store(y + (static_cast<long long>(t) * nvec + c) * VEC);
     }
-    P v;
-#pragma unroll
-    for (int q = 0; q < VEC; ++q) v.v[q] = E::from_float(acc[q]);
-    *reinterpret_cast<P*>(y + (t * nvec + c) * VEC) = v;
   }
 }
 
-// One block a token: its gradient row times each weight to the rows' gradients, and its dot
-// product with each row to the weights' gradients.
-constexpr int kBackThreads = 256;
+// One block a token: its gradient row times each weight to the rows' gradients, and its dot product
+// with each row to the weights' gradients, four rows at a time (eight take 72 registers, and the
+// three blocks that then fit on an SM are too few to cover the latency: 88 us against 77 us at 8191
+// tokens x 6 rows of 4 KB).
+constexpr int kBackRows = 4;
 
 template <class E, int VEC>
-__global__ void __launch_bounds__(kBackThreads)
+__global__ void __launch_bounds__(kRowThreads, 5)
     combine_backward_kernel(const typename E::T* rows, const typename E::T* grad,
                             long long grad_stride, const int* position, const float* weights,
                             const int* live, typename E::T* d_rows, float* d_weights, int tokens,
                             int k, int nvec) {
   using P = Pack<E, VEC>;
-  __shared__ float part[kBackThreads / 32];
+  __shared__ float part[kRowThreads / 32][kBackRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long n = static_cast<long long>(tokens) * k;
   for (long long t = blockIdx.x; t < tokens; t += gridDim.x) {
     const typename E::T* g = grad + t * grad_stride;
-    for (int j = 0; j < k; ++j) {
-      const int at = position[t * k + j];
-      const bool ok = at >= 0 && at < n;
-      float dot = 0.0f;
-      if (ok) {
-        const float w = weights ? weights[t * k + j] : 1.0f;
-        for (int c = threadIdx.x; c < nvec; c += blockDim.x) {
-          const P gv = *reinterpret_cast<const P*>(g + static_cast<long long>(c) * VEC);
-          const long long to = (static_cast<long long>(at) * nvec + c) * VEC;
-          P o;
+    for (int j0 = 0; j0 < k; j0 += kBackRows) {
+      int at[kBackRows];
+      float w[kBackRows], dot[kBackRows];
 #pragma unroll
-          for (int q = 0; q < VEC; ++q) o.v[q] = E::from_float(w * E::to_float(gv.v[q]));
-          if (d_weights) {
-            const P rv = *reinterpret_cast<const P*>(rows + to);
+      for (int u = 0; u < kBackRows; ++u) {
+        const int a = j0 + u < k ? position[t * k + j0 + u] : -1;
+        at[u] = a >= 0 && a < n ? a : -1;
+        w[u] = at[u] >= 0 && weights ? weights[t * k + j0 + u] : 1.0f;
+        dot[u] = 0.0f;
+      }
+      for (int c = threadIdx.x; c < nvec; c += blockDim.x) {
+        float gv[VEC];
+        P::load(g + static_cast<long long>(c) * VEC).get(gv);
+#pragma unroll
+        for (int h = 0; h < kBackRows; h += kAhead) {
+          P r[kAhead];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const bool in = d_weights && at[h + u] >= 0;
+            r[u] = in ? P::load(rows + (static_cast<long long>(at[h + u]) * nvec + c) * VEC)
+                      : zero_pack<E, VEC>();
+          }
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            if (j0 + h + u >= k) break;
+            float rv[VEC], ov[VEC];
+            r[u].get(rv);
 #pragma unroll
             for (int q = 0; q < VEC; ++q) {
-              dot = fmaf(E::to_float(gv.v[q]), E::to_float(rv.v[q]), dot);
+              dot[h + u] = fmaf(gv[q], rv[q], dot[h + u]);
+              ov[q] = w[h + u] * gv[q];
+            }
+            if (d_rows && at[h + u] >= 0) {
+              P o;
+              o.set(ov);
+              o.store(d_rows + (static_cast<long long>(at[h + u]) * nvec + c) * VEC);
             }
           }
-          if (d_rows) *reinterpret_cast<P*>(d_rows + to) = o;
         }
       }
       if (d_weights) {
-        dot = warp_sum(dot);
-        if (lane == 0) part[warp] = dot;
+#pragma unroll
+        for (int u = 0; u < kBackRows; ++u) {
+          dot[u] = warp_sum(dot[u]);
+          if (lane == 0) part[warp][u] = dot[u];
+        }
         __syncthreads();
-        if (threadIdx.x == 0) {
+        if (threadIdx.x < kBackRows && j0 + threadIdx.x < static_cast<unsigned>(k)) {
           float sum = 0.0f;
-          for (int i = 0; i < static_cast<int>(blockDim.x / 32); ++i) sum += part[i];
-          d_weights[t * k + j] = sum;
+          for (int i = 0; i < static_cast<int>(blockDim.x / 32); ++i) sum += part[i][threadIdx.x];
+          d_weights[t * k + j0 + threadIdx.x] = sum;
         }
         __syncthreads();
       }
@@ -482,11 +880,8 @@ __global__ void __launch_bounds__(kBackThreads)
     const int first = *live;
     for (long long r = (first < 0 ? 0 : first) + static_cast<long long>(blockIdx.x); r < n;
          r += gridDim.x) {
-      P z;
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) z.v[q] = E::from_float(0.0f);
       for (int c = threadIdx.x; c < nvec; c += blockDim.x) {
-        *reinterpret_cast<P*>(d_rows + (r * nvec + c) * VEC) = z;
+        zero_pack<E, VEC>().store(d_rows + (r * nvec + c) * VEC);
       }
     }
   }
@@ -496,51 +891,39 @@ __global__ void __launch_bounds__(kBackThreads)
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-int sm_count(int* out) {
-  static int known[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (known[dev] == 0) {
-    e = cudaDeviceGetAttribute(&known[dev], cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return e;
-  }
-  *out = known[dev];
-  return 0;
-}
+std::mutex g_mu;  // over what is looked up once per device
 
+// The kernel whose lanes own 1, 2, 4, 8, 16 or 32 experts each, wide where the rows allow it.
 template <class E, int NPL>
 int launch_route(const RouteParams& p, cudaStream_t s) {
-  route_kernel<E, NPL><<<(p.tokens + 3) / 4, 128, 0, s>>>(p);
+  using T = typename E::T;
+  constexpr int kPer = 16 / sizeof(T) < NPL ? 16 / sizeof(T) : NPL;
+  const bool wide = p.num == 32 * NPL && p.stride % kPer == 0 && aligned(p.logits, sizeof(T) * kPer);
+  const int grid = (p.tokens + kRouteWarps - 1) / kRouteWarps;
+  if (wide) route_kernel<E, NPL, true><<<grid, 32 * kRouteWarps, 0, s>>>(p);
+  else route_kernel<E, NPL, false><<<grid, 32 * kRouteWarps, 0, s>>>(p);
   return cudaGetLastError();
 }
 template <class E, int NPL>
-int launch_route_back(const RouteBackParams& p, cudaStream_t s) {
-  route_backward_kernel<E, NPL><<<(p.tokens + 3) / 4, 128, 0, s>>>(p);
+int launch_route(const RouteBackParams& p, cudaStream_t s) {
+  using T = typename E::T;
+  constexpr int kPer = 16 / sizeof(T) < NPL ? 16 / sizeof(T) : NPL;
+  const bool wide = p.num == 32 * NPL && p.stride % kPer == 0 &&
+                    aligned(p.logits, sizeof(T) * kPer) && aligned(p.d_logits, sizeof(T) * kPer);
+  const int grid = (p.tokens + kRouteWarps - 1) / kRouteWarps;
+  if (wide) route_backward_kernel<E, NPL, true><<<grid, 32 * kRouteWarps, 0, s>>>(p);
+  else route_backward_kernel<E, NPL, false><<<grid, 32 * kRouteWarps, 0, s>>>(p);
   return cudaGetLastError();
 }
 
-// Index of the kernel whose lanes own 1, 2, 4, 8, 16 or 32 experts each.
-int lane_class(int num) {
-  int c = 0;
-  while ((32 << c) < num) ++c;
-  return c;
-}
-
-template <class E>
-int route_of(const RouteParams& p, cudaStream_t s) {
-  constexpr int (*kBy[])(const RouteParams&, cudaStream_t) = {
-      launch_route<E, 1>, launch_route<E, 2>,  launch_route<E, 4>,
-      launch_route<E, 8>, launch_route<E, 16>, launch_route<E, 32>};
-  return kBy[lane_class(p.num)](p, s);
-}
-template <class E>
-int route_back_of(const RouteBackParams& p, cudaStream_t s) {
-  constexpr int (*kBy[])(const RouteBackParams&, cudaStream_t) = {
-      launch_route_back<E, 1>, launch_route_back<E, 2>,  launch_route_back<E, 4>,
-      launch_route_back<E, 8>, launch_route_back<E, 16>, launch_route_back<E, 32>};
-  return kBy[lane_class(p.num)](p, s);
+template <class E, class P>
+int route_of(const P& p, cudaStream_t s) {
+  if (p.num <= 32) return launch_route<E, 1>(p, s);
+  if (p.num <= 64) return launch_route<E, 2>(p, s);
+  if (p.num <= 128) return launch_route<E, 4>(p, s);
+  if (p.num <= 256) return launch_route<E, 8>(p, s);
+  if (p.num <= 512) return launch_route<E, 16>(p, s);
+  return launch_route<E, 32>(p, s);
 }
 
 template <class F>
@@ -556,15 +939,19 @@ int by_elem(int elem, F f) {
 size_t elem_size(int elem) { return elem == BT_ELEM_F32 ? 4 : 2; }
 bool elem_ok(int elem) { return elem == BT_ELEM_F16 || elem == BT_ELEM_BF16 || elem == BT_ELEM_F32; }
 
-int grid_for(long long items, int threads, int sms) {
-  const long long want = (items + threads - 1) / threads;
-  const long long most = static_cast<long long>(sms) * (2048 / threads);
-  return static_cast<int>(want < most ? (want > 0 ? want : 1) : most);
+// Threads over a row's vectors, a power of two, and rows side by side to fill the block.
+dim3 row_block(int nvec) {
+  int x = 32;
+  while (x < nvec && x < kRowThreads) x *= 2;
+  return dim3(x, kRowThreads / x);
 }
+// Blocks for `rows` rows, `per` of them a block: the scheduler evens them out over the SMs better
+// than a grid of resident blocks that stride over the rows (a sixth slower where 6 of 8 fit).
+int row_grid(long long rows, int per) { return static_cast<int>((rows + per - 1) / per); }
 
 bool rows_ok(int tokens, int k, int width) {
   return tokens > 0 && k > 0 && k <= BT_MAX_EXPERTS_PER_TOKEN && width > 0 &&
-         static_cast<long long>(tokens) * k <= 0x7FFFFFFFll;
+         static_cast<long long>(tokens) * k <= BT_MAX_ASSIGNMENTS;
 }
 
 // Whether 16-byte accesses are possible for this width, these strides and these pointers.
@@ -572,6 +959,39 @@ bool wide(int elem, int width, long long stride, const void* a, const void* b, c
   const int per = static_cast<int>(16 / elem_size(elem));
   return width % per == 0 && stride % per == 0 && aligned(a, 16) && aligned(b, 16) &&
          aligned(c, 16);
+}
+
+size_t order_smem(int experts, long long per_block) {
+  const long long tile = per_block < kTile ? per_block : kTile;
+  return sizeof(uint32_t) * (kOrderWarps * experts + 3 * experts + 32) +
+         sizeof(uint16_t) * static_cast<size_t>(tile);
+}
+
+// Blocks, and a block's entries: one block while its threads take four entries each.
+int order_blocks(int n, int* per_block) {
+  long long per = kOrderRun;
+  if (n > static_cast<long long>(kOrderRun) * kOrderBlocks) {
+    per = (n + kOrderBlocks * 1024ll - 1) / (kOrderBlocks * 1024ll) * 1024;
+  }
+  *per_block = static_cast<int>(per);
+  return static_cast<int>((n + per - 1) / per);
+}
+
+// Once per device: shared memory beyond the default.
+int order_ready() {
+  static bool known[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(g_mu);
+  if (!known[dev]) {
+    e = cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(order_smem(BT_MAX_EXPERTS, kTile)));
+    if (e != cudaSuccess) return e;
+    known[dev] = true;
+  }
+  return 0;
 }
 
 }  // namespace bte
@@ -615,39 +1035,48 @@ int bt_route_backward(const void* d_logits, int elem, int tokens, int experts, l
   RouteBackParams p{d_logits, stride, d_experts, d_grad, d_logits_grad, tokens, experts, k,
                     score == BT_SCORE_SIGMOID, renormalize != 0, scale};
   return by_elem(elem, [&](auto e) {
-    return route_back_of<decltype(e)>(p, static_cast<cudaStream_t>(stream));
+    return route_of<decltype(e)>(p, static_cast<cudaStream_t>(stream));
   });
 }
 
+size_t bt_expert_order_workspace_size(int n, int experts) {
+  if (n <= 0 || n > BT_MAX_ASSIGNMENTS || experts <= 0 || experts > BT_MAX_EXPERTS) return 0;
+  int per = 0;
+  const int blocks = bte::order_blocks(n, &per);
+  return (sizeof(uint32_t) * static_cast<size_t>(blocks) * experts + 255) / 256 * 256;
+}
+
 int bt_expert_order(const int* d_experts, int n, int experts, int* d_offsets, int* d_order,
-                    int* d_position, void* stream) {
+                    int* d_position, void* d_workspace, size_t workspace_bytes, void* stream) {
   using namespace bte;
-  if (n <= 0 || experts <= 0 || experts > BT_MAX_EXPERTS) return cudaErrorInvalidValue;
-  if (!d_experts || !d_offsets || !d_order || !d_position || !aligned(d_experts, 4) ||
-      !aligned(d_offsets, 4) || !aligned(d_order, 4) || !aligned(d_position, 4)) {
+  const size_t need = bt_expert_order_workspace_size(n, experts);
+  if (need == 0 || workspace_bytes < need) return cudaErrorInvalidValue;
+  if (!d_experts || !d_offsets || !d_order || !d_position || !d_workspace ||
+      !aligned(d_experts, 4) || !aligned(d_offsets, 4) || !aligned(d_order, 4) ||
+      !aligned(d_position, 4) || !aligned(d_workspace, 16)) {
     return cudaErrorInvalidValue;
   }
-  int blocks = 1;
-  while (blocks < 8 && static_cast<long long>(blocks) * kOrderThreads * 4 < n) blocks *= 2;
-  const long long warps = static_cast<long long>(blocks) * kOrderWarps;
-  const int per_warp = static_cast<int>(((n + warps - 1) / warps + 31) / 32 * 32);
-  OrderParams p{d_experts, d_offsets, d_order, d_position, n, experts, per_warp};
-  const size_t smem = sizeof(uint32_t) * (kOrderWarps * experts + 2 * experts + 32);
-  cudaError_t e = cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem));
-  if (e != cudaSuccess) return e;
+  if (const int rc = order_ready()) return rc;
+  OrderParams p{d_experts, d_offsets, d_order, d_position, static_cast<uint32_t*>(d_workspace), n,
+                experts, 0};
+  const int blocks = order_blocks(n, &p.per_block);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(kOrderThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.dynamicSmemBytes = order_smem(experts, p.per_block);
+  cfg.stream = s;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = blocks;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  if (blocks > 1) {
+    // the second kernel may start while the first runs, and waits for its counts
+    order_count_kernel<<<blocks, kOrderThreads, sizeof(uint32_t) * experts, s>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
   return cudaLaunchKernelEx(&cfg, order_kernel, p);
 }
 
@@ -659,22 +1088,20 @@ int bt_dispatch(const void* d_x, int elem, int tokens, int k, int width, long lo
       !aligned(d_rows, elem_size(elem)) || !aligned(d_order, 4)) {
     return cudaErrorInvalidValue;
   }
-  int sms = 0;
-  if (const int rc = sm_count(&sms)) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return by_elem(elem, [&](auto e) -> int {
     using E = decltype(e);
     using T = typename E::T;
     constexpr int kWide = 16 / sizeof(T);
-    const long long rows = static_cast<long long>(tokens) * k;
-    if (wide(elem, width, stride, d_x, d_rows, nullptr)) {
-      const int nvec = width / kWide;
-      dispatch_kernel<E, kWide><<<grid_for(rows * nvec, 256, sms), 256, 0, s>>>(
-          static_cast<const T*>(d_x), stride, d_order, static_cast<T*>(d_rows), tokens, k, nvec);
-    } else {
-      dispatch_kernel<E, 1><<<grid_for(rows * width, 256, sms), 256, 0, s>>>(
-          static_cast<const T*>(d_x), stride, d_order, static_cast<T*>(d_rows), tokens, k, width);
-    }
+    const int n = tokens * k;
+    const bool w = wide(elem, width, stride, d_x, d_rows, nullptr);
+    const int nvec = w ? width / kWide : width;
+    const dim3 block = row_block(nvec);
+    const int grid = row_grid(n, static_cast<int>(block.y) * kAhead);
+    const T* x = static_cast<const T*>(d_x);
+    T* rows = static_cast<T*>(d_rows);
+    if (w) dispatch_kernel<E, kWide><<<grid, block, 0, s>>>(x, stride, d_order, rows, n, k, nvec);
+    else dispatch_kernel<E, 1><<<grid, block, 0, s>>>(x, stride, d_order, rows, n, k, nvec);
     return cudaGetLastError();
   });
 }
@@ -687,20 +1114,21 @@ int bt_combine(const void* d_rows, int elem, int tokens, int k, int width, const
       !aligned(d_y, elem_size(elem)) || !aligned(d_position, 4) || !aligned(d_weights, 4)) {
     return cudaErrorInvalidValue;
   }
-  int sms = 0;
-  if (const int rc = sm_count(&sms)) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return by_elem(elem, [&](auto e) -> int {
     using E = decltype(e);
     using T = typename E::T;
     constexpr int kWide = 16 / sizeof(T);
-    if (wide(elem, width, 0, d_rows, d_y, nullptr)) {
-      const int nvec = width / kWide;
-      combine_kernel<E, kWide><<<grid_for(static_cast<long long>(tokens) * nvec, 256, sms), 256, 0, s>>>(
-          static_cast<const T*>(d_rows), d_position, d_weights, static_cast<T*>(d_y), tokens, k, nvec);
+    const bool w = wide(elem, width, 0, d_rows, d_y, nullptr);
+    const int nvec = w ? width / kWide : width;
+    const dim3 block = row_block(nvec);
+    const int grid = row_grid(tokens, static_cast<int>(block.y));
+    const T* rows = static_cast<const T*>(d_rows);
+    T* y = static_cast<T*>(d_y);
+    if (w) {
+      combine_kernel<E, kWide><<<grid, block, 0, s>>>(rows, d_position, d_weights, y, tokens, k, nvec);
     } else {
-      combine_kernel<E, 1><<<grid_for(static_cast<long long>(tokens) * width, 256, sms), 256, 0, s>>>(
-          static_cast<const T*>(d_rows), d_position, d_weights, static_cast<T*>(d_y), tokens, k, width);
+      combine_kernel<E, 1><<<grid, block, 0, s>>>(rows, d_position, d_weights, y, tokens, k, nvec);
     }
     return cudaGetLastError();
   });
@@ -719,24 +1147,23 @@ int bt_combine_backward(const void* d_rows, const void* d_grad, int elem, int to
       !aligned(d_weights_grad, 4)) {
     return cudaErrorInvalidValue;
   }
-  int sms = 0;
-  if (const int rc = sm_count(&sms)) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return by_elem(elem, [&](auto e) -> int {
     using E = decltype(e);
     using T = typename E::T;
     constexpr int kWide = 16 / sizeof(T);
-    const int grid = grid_for(static_cast<long long>(tokens) * kBackThreads, kBackThreads, sms);
     const T *rows = static_cast<const T*>(d_rows), *grad = static_cast<const T*>(d_grad);
     T* d_r = static_cast<T*>(d_rows_grad);
-    if (wide(elem, width, grad_stride, d_rows, d_grad, d_rows_grad)) {
-      combine_backward_kernel<E, kWide><<<grid, kBackThreads, 0, s>>>(
-          rows, grad, grad_stride, d_position, d_weights, d_live, d_r, d_weights_grad, tokens, k,
-          width / kWide);
+    const bool w = wide(elem, width, grad_stride, d_rows, d_grad, d_rows_grad);
+    const int nvec = w ? width / kWide : width;
+    const int threads = static_cast<int>(row_block(nvec).x);
+    const int grid = row_grid(tokens, 1);
+    if (w) {
+      combine_backward_kernel<E, kWide><<<grid, threads, 0, s>>>(
+          rows, grad, grad_stride, d_position, d_weights, d_live, d_r, d_weights_grad, tokens, k, nvec);
     } else {
-      combine_backward_kernel<E, 1><<<grid, kBackThreads, 0, s>>>(
-          rows, grad, grad_stride, d_position, d_weights, d_live, d_r, d_weights_grad, tokens, k,
-          width);
+      combine_backward_kernel<E, 1><<<grid, threads, 0, s>>>(
+          rows, grad, grad_stride, d_position, d_weights, d_live, d_r, d_weights_grad, tokens, k, nvec);
     }
     return cudaGetLastError();
   });

@@ -1267,7 +1267,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(Params p
   u64 best = 0;
   float total = k.z;
   // +inf or NaN logits (and products out of range): no approximate sums
-  bool passes = !(k.z < INFINITY) || k.m == INFINITY;
+  bool passes = !(k.z > 0.5f && k.z < INFINITY) || k.m == INFINITY;
   if (!passes && (by_k || by_p) && !one) {
     // p alone starts from about 64 elements, which most rows' nuclei are within
     const uint32_t want = by_k ? static_cast<uint32_t>(k.top_k) : 64u;

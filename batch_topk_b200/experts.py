@@ -18,8 +18,9 @@ from typing import NamedTuple
 
 import torch
 
-from . import MAX_EXPERTS, MAX_EXPERTS_PER_TOKEN, SCORE_SIGMOID, SCORE_SOFTMAX, _lib
-from .sampling import ELEM, launch
+from . import (MAX_ASSIGNMENTS, MAX_EXPERTS, MAX_EXPERTS_PER_TOKEN, SCORE_SIGMOID, SCORE_SOFTMAX,
+               _lib)
+from .sampling import ELEM, launch, raw_stream
 
 SCORES = {"softmax": SCORE_SOFTMAX, "sigmoid": SCORE_SIGMOID}
 
@@ -34,6 +35,19 @@ class ExpertOrder(NamedTuple):
     offsets: torch.Tensor
     order: torch.Tensor
     position: torch.Tensor
+
+
+_workspaces: dict = {}
+
+
+def _workspace(device, nbytes):
+    """Scratch of the device's current stream, grown as needed: calls on one stream run in order,
+    so they may share it; calls on different streams never do."""
+    key = (device.index, raw_stream(device.index))
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _workspaces[key] = torch.empty(max(nbytes, 1 << 18), dtype=torch.uint8, device=device)
+    return ws
 
 
 def _first_order(grad):
@@ -137,8 +151,8 @@ def expert_order(experts: torch.Tensor, num_experts: int) -> ExpertOrder:
     if not 1 <= num_experts <= MAX_EXPERTS:
         raise ValueError(f"1 to {MAX_EXPERTS} experts are supported, got {num_experts}")
     n = experts.numel()
-    if n > 2**31 - 1:
-        raise ValueError(f"at most 2^31 - 1 assignments are supported, got {n}")
+    if n > MAX_ASSIGNMENTS:
+        raise ValueError(f"at most {MAX_ASSIGNMENTS} assignments are supported, got {n}")
     dev = experts.device
     experts = experts.contiguous()
     if n == 0:
@@ -148,8 +162,10 @@ def expert_order(experts: torch.Tensor, num_experts: int) -> ExpertOrder:
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
     order = torch.empty(n, dtype=torch.int32, device=dev)
     position = torch.empty_like(experts)
-    launch("expert_order", _lib.load().bt_expert_order, dev, experts.data_ptr(), n, num_experts,
-           offsets.data_ptr(), order.data_ptr(), position.data_ptr())
+    lib = _lib.load()
+    ws = _workspace(dev, lib.bt_expert_order_workspace_size(n, num_experts))
+    launch("expert_order", lib.bt_expert_order, dev, experts.data_ptr(), n, num_experts,
+           offsets.data_ptr(), order.data_ptr(), position.data_ptr(), ws.data_ptr(), ws.numel())
     return ExpertOrder(offsets, order, position)
 
 
@@ -161,8 +177,9 @@ def _check_plan(plan, device, tokens=None, rows=None):
     n, k = position.shape
     if order.numel() != n * k or offsets.numel() < 2:
         raise ValueError("plan.order must hold one place for each entry of plan.position")
-    if not 1 <= k <= MAX_EXPERTS_PER_TOKEN:
-        raise ValueError(f"1 to {MAX_EXPERTS_PER_TOKEN} experts a token are supported, got {k}")
+    if not 1 <= k <= MAX_EXPERTS_PER_TOKEN or n * k > MAX_ASSIGNMENTS:
+        raise ValueError(f"1 to {MAX_EXPERTS_PER_TOKEN} experts a token and at most "
+                         f"{MAX_ASSIGNMENTS} assignments are supported, got {n} x {k}")
     if tokens is not None and tokens != n:
         raise ValueError(f"the plan is for {n} tokens, x has {tokens}")
     if rows is not None and rows != n * k:

@@ -16,7 +16,7 @@ from . import BatchTopkError, ELEM_BF16, ELEM_F16, ELEM_F32, MAX_SEG_LEN, _lib
 ELEM = {torch.float16: ELEM_F16, torch.bfloat16: ELEM_BF16, torch.float32: ELEM_F32}
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream without its wrapper object
+raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream without its wrapper object
 
 
 def launch(what, entry, device, *args):
@@ -24,10 +24,10 @@ def launch(what, entry, device, *args):
     object cost microseconds, which small calls feel: neither is made when it is not needed."""
     index = device.index
     if index == torch.cuda.current_device():
-        rc = entry(*args, _raw_stream(index))
+        rc = entry(*args, raw_stream(index))
     else:
         with torch.cuda.device(device):  # the library launches on the current device
-            rc = entry(*args, _raw_stream(index))
+            rc = entry(*args, raw_stream(index))
     if rc != 0:
         raise BatchTopkError(rc, what)
 

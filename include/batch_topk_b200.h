@@ -177,8 +177,8 @@ int bt_logits_topk_status(const void* d_workspace, int M, int V, int D, int k, v
 /* Operators of a language model built on selection; no reference counterpart (the reference
  * selects and stops, include/batch_topk.cuh:10-19).  Common to all of them: `elem` names the type
  * of the values (BT_ELEM_*), strides count elements between rows (the values of a row are
- * adjacent), pointers are aligned to their elements, a call is asynchronous on `stream` and needs
- * no workspace, and cudaErrorInvalidValue answers a bad shape, a NULL or misaligned pointer or an
+ * adjacent), pointers are aligned to their elements, a call is asynchronous on `stream` and
+ * needs no workspace (but bt_expert_order), and cudaErrorInvalidValue answers a bad shape, a NULL or misaligned pointer or an
  * unknown constant before anything is launched. */
 #define BT_ELEM_F16 0
 #define BT_ELEM_BF16 1
@@ -214,6 +214,7 @@ int bt_sample(const void* d_logits, int elem, int rows, int vocab, long long log
 
 #define BT_MAX_EXPERTS 1024
 #define BT_MAX_EXPERTS_PER_TOKEN 32
+#define BT_MAX_ASSIGNMENTS (1 << 30) /* tokens * k of the calls on assignments and their rows */
 #define BT_SCORE_SOFTMAX 0
 #define BT_SCORE_SIGMOID 1
 
@@ -244,9 +245,13 @@ int bt_route_backward(const void* d_logits, int elem, int tokens, int experts, l
 /* The n assignments (expert numbers, e.g. bt_route's [tokens, k] read row by row) sorted by expert,
  * equal experts in input order: expert e's are d_order[d_offsets[e] .. d_offsets[e + 1]), each an
  * index into d_experts; d_position is the inverse.  Numbers outside [0, experts) are left out:
- * their d_position is -1, and d_order ends with as many -1.  d_offsets holds experts + 1 values. */
+ * their d_position is -1, and d_order ends with as many -1.  d_offsets holds experts + 1 values.
+ * The workspace (16-byte aligned, no initialisation needed) is sized by
+ * bt_expert_order_workspace_size, which is 0 for an unsupported shape. */
 int bt_expert_order(const int* d_experts, int n, int experts, int* d_offsets, int* d_order,
-                    int* d_position, void* stream);
+                    int* d_position, void* d_workspace, size_t workspace_bytes, void* stream);
+
+size_t bt_expert_order_workspace_size(int n, int experts);
 
 /* Rows of x [tokens, width] in the experts' order: d_rows[p] = x[d_order[p] / k], and zeros where
  * d_order[p] is -1 (or not below tokens * k).  d_rows is [tokens * k, width]. */

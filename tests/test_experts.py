@@ -199,7 +199,8 @@ def make_experts(tokens, k, num, seed, popular=False):
 @pytest.mark.gpu
 @pytest.mark.parametrize("tokens,k,num", [(1, 1, 1), (1, 8, 256), (3, 2, 5), (31, 1, 1024),
                                           (33, 8, 64), (1000, 6, 160), (4099, 8, 256),
-                                          (40000, 4, 1024), (65521, 8, 8), (100003, 7, 511)])
+                                          (40000, 4, 1024), (65521, 8, 8), (100003, 7, 511),
+                                          (1400003, 6, 33)])
 @pytest.mark.parametrize("popular", [False, True])
 def test_expert_order(tokens, k, num, popular):
     e = make_experts(tokens, k, num, tokens + num, popular)
@@ -412,11 +413,17 @@ def test_abi_argument_errors():
                dict(score=9), dict(o=FAKE + 1), dict(g=FAKE + 2)):
         assert back(**kw) == INVALID, kw
 
-    def order(e=FAKE, n=8, num=4, off=FAKE, o=FAKE, pos=FAKE):
-        return bt.expert_order(e, n, num, off, o, pos)
+    need = bt.expert_order_workspace_size(8, 4)
+    assert need > 0 and need % 256 == 0
+    assert bt.expert_order_workspace_size(0, 4) == 0 and bt.expert_order_workspace_size(8, 0) == 0
+    assert bt.expert_order_workspace_size(bt.MAX_ASSIGNMENTS + 1, 4) == 0
+    assert bt.expert_order_workspace_size(8, bt.MAX_EXPERTS + 1) == 0
+
+    def order(e=FAKE, n=8, num=4, off=FAKE, o=FAKE, pos=FAKE, ws=FAKE, wsb=need):
+        return bt.expert_order(e, n, num, off, o, pos, ws, wsb)
 
     for kw in (dict(e=0), dict(n=0), dict(num=0), dict(num=1025), dict(off=0), dict(o=0),
-               dict(pos=0), dict(pos=FAKE + 2)):
+               dict(pos=0), dict(pos=FAKE + 2), dict(ws=0), dict(ws=FAKE + 8), dict(wsb=need - 1)):
         assert order(**kw) == INVALID, kw
 
     def disp(x=FAKE, elem=0, t=4, k=2, width=8, stride=8, o=FAKE, r=FAKE):

@@ -125,6 +125,20 @@ def test_masked_rows(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e5, 3e8, 1e9, 1e12, 1e30])
+@pytest.mark.parametrize("temperature", [1.0, 1e-3, 1e4])
+def test_huge_logits(size, temperature):
+    """Logits far from zero: sums of weights are relative to the maximum, however large it is."""
+    x, q = inputs(6, 4099, "fp32", 15, size)
+    x[3:] += size * 4
+    x[5] = -size
+    for kw in (dict(), dict(top_k=9), dict(top_p=0.9), dict(min_p=0.1), dict(temperature=0.0)):
+        kw = {"temperature": temperature, **kw}
+        tokens, logprobs = api.sample(x, q, **kw)
+        check(x, q, tokens, logprobs, **kw)
+
+
+@pytest.mark.gpu
 def test_settings_of_each_row():
     """One value a row, those outside their range among them: they switch the filter off or clamp."""
     n = 24
