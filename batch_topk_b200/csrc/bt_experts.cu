@@ -127,18 +127,24 @@ __device__ __forceinline__ float warp_max(float v) {  // no NaN
   return r;
 }
 
-// Values of the warp sorted across its lanes, largest first.
+// Values of the warp sorted across its lanes, largest first.  Runs that have to be sorted the other
+// way hold negated values meanwhile, so that every exchange goes by one bit of the lane.
 __device__ __forceinline__ float warp_sort_down(float v) {
-  const int lane = threadIdx.x & 31;
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t bits = __float_as_uint(v);
 #pragma unroll
-  for (int size = 2; size <= 32; size <<= 1) {
+  for (int log = 1; log <= 5; ++log) {
+    // negated in stage log: lanes with bit `log`; it was bit log - 1 in the stage before
+    const uint32_t flip = log == 1 ? lane >> 1 : (log == 5 ? lane >> 4 : (lane >> log) ^ (lane >> (log - 1)));
+    bits ^= flip << 31;
 #pragma unroll
-    for (int d = size >> 1; d > 0; d >>= 1) {
-      const float o = __shfl_xor_sync(kAll, v, d);
-      v = ((lane & d) == 0) == ((lane & size) == 0) ? fmaxf(v, o) : fminf(v, o);
+    for (int d = 1 << (log - 1); d > 0; d >>= 1) {
+      const float a = __uint_as_float(bits);
+      const float o = __shfl_xor_sync(kAll, a, d);
+      bits = __float_as_uint((lane & d) ? fminf(a, o) : fmaxf(a, o));
     }
   }
-  return v;
+  return __uint_as_float(bits);
 }
 
 // The lane's logits: NaN reads as -inf, and so does every place past the last expert.  WIDE: the
@@ -269,8 +275,8 @@ __device__ __forceinline__ void close_groups(const RouteParams& p, const float (
 
 template <class E, int NPL, bool WIDE>
 __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) {
-  __shared__ unsigned long long found[kRouteWarps][32];  // candidates, see place_key
-  __shared__ float rows[kRouteWarps][32 * NPL];
+  __shared__ __align__(16) unsigned long long found[kRouteWarps][32];  // candidates, see place_key
+  __shared__ __align__(16) float rows[kRouteWarps][32 * NPL];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + warp;
   if (t >= p.tokens) return;
@@ -291,9 +297,10 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) 
   const bool grouped = p.groups > 1;
   const bool near = p.bias && p.sigmoid && !grouped;  // c within 1e-6 first, exact for candidates
 #pragma unroll
-  for (int i = 0; i < NPL; ++i) {
-    c[i] = x[i];
-    if (p.bias) {
+  for (int i = 0; i < NPL; ++i) c[i] = x[i];
+  if (p.bias) {
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
       const int e = lane * NPL + i;
       const float b = e < p.num ? p.bias[e] : 0.0f;
       const float s = near ? sigmoid_near(x[i]) : score_of(x[i]);
@@ -320,9 +327,10 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) 
   float bound = __shfl_sync(kAll, sorted, p.k - 1);
   if (near) bound -= 4e-6f + 1e-6f * fabsf(bound);
   bound = fmaxf(bound, -3.402823466e38f);  // closed experts are below every bound
-  int own = 0;
+  uint32_t mask = 0;  // this lane's candidates
 #pragma unroll
-  for (int i = 0; i < NPL; ++i) own += c[i] >= bound;
+  for (int i = 0; i < NPL; ++i) mask |= c[i] >= bound ? 1u << i : 0u;
+  const int own = __popc(mask);
   int at = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -333,11 +341,14 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) 
   at -= own;
   int expert = -1;  // slot `lane`
   if (n <= 32) {
-    if (own) {
+    found[warp][lane] = 0;  // behind every candidate
+    float* mine_of = rows[warp] + lane * NPL;  // indexed by a variable, which registers cannot be
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) {
-        if (c[i] >= bound) found[warp][at++] = place_key(c[i], lane * NPL + i);
-      }
+    for (int i = 0; i < NPL; ++i) mine_of[i] = c[i];
+    __syncwarp();
+    for (; mask; mask &= mask - 1) {
+      const int i = __ffs(mask) - 1;
+      found[warp][at++] = place_key(mine_of[i], lane * NPL + i);
     }
     __syncwarp();
     unsigned long long mine = 0;
@@ -355,7 +366,13 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) 
       __syncwarp();
     }
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += found[warp][j] > mine;
+    for (int j = 0; j < n; j += 4) {
+#pragma unroll
+      for (int u = 0; u < 4; u += 2) {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&found[warp][j + u]);
+        rank += (two.x > mine) + (two.y > mine);
+      }
+    }
     __syncwarp();
     if (lane < n) found[warp][rank] = mine;
     __syncwarp();
@@ -411,7 +428,7 @@ struct RouteBackParams {
 //   softmax: dx_i = s_i (ds_i - sum_j ds_j s_j) everywhere.
 // Each lane writes its own run first; the chosen experts' values then replace theirs.
 template <class E, int NPL, bool WIDE>
-__global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(RouteBackParams p) {
+__global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 8 ? 16 : 1) route_backward_kernel(RouteBackParams p) {
   using T = typename E::T;
   constexpr int kPer = 16 / sizeof(T) < NPL ? 16 / sizeof(T) : NPL;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -419,17 +436,20 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(RouteB
   if (t >= p.tokens) return;
   const T* row = static_cast<const T*>(p.logits) + t * p.stride;
   T* out = static_cast<T*>(p.d_logits) + t * static_cast<long long>(p.num);
-  int e = lane < p.k ? p.experts[t * p.k + lane] : -1;
-  if (e >= p.num) e = -1;
-  const float g = e >= 0 ? p.scale * p.grad[t * p.k + lane] : 0.0f;
-  const float xe = e >= 0 ? fmaxf(E::to_float(row[e]), kNegInf) : kNegInf;
   float x[NPL], m = 0.0f, z = 1.0f, se, one_minus = 0.0f;
+  if (!p.sigmoid) load_logits<E, NPL, WIDE>(row, p.num, x);
+  int e = lane < p.k ? p.experts[t * p.k + lane] : -1;
+  float g = lane < p.k ? p.scale * p.grad[t * p.k + lane] : 0.0f;
+  if (e < 0 || e >= p.num) {
+    e = -1;
+    g = 0.0f;
+  }
+  const float xe = e >= 0 ? fmaxf(E::to_float(row[e]), kNegInf) : kNegInf;
   if (p.sigmoid) {
     const float u = expf(-fabsf(xe));
     se = sigmoid_rn(xe);
     one_minus = xe > 0.0f ? u / (1.0f + u) : 1.0f / (1.0f + u);
   } else {
-    load_logits<E, NPL, WIDE>(row, p.num, x);
     m = warp_max(row_max(x));
     z = row_sum(x, m);
     se = __fdiv_rn(exp_below(xe, m), z);
@@ -804,7 +824,7 @@ __global__ void __launch_bounds__(kRowThreads)
 
 // One block a token: its gradient row times each weight to the rows' gradients, and its dot product
 // with each row to the weights' gradients, four rows at a time (eight take 72 registers, and the
-// three blocks that then fit on an SM are too few to cover the latency: 88 us against 77 us at 8191
+// three blocks that then fit on an SM are too few to cover the latency: 90 us against 79 us at 8191
 // tokens x 6 rows of 4 KB).
 constexpr int kBackRows = 4;
 
