@@ -9,7 +9,7 @@ import ctypes as C
 import os
 import threading
 
-from .build import LIB
+from .build import LIB, TENSORS
 
 EXPORTED = (
     "bt_topk_half",
@@ -52,6 +52,23 @@ _lib = None
 
 class LibraryMissing(RuntimeError):
     pass
+
+
+_tensors = None
+
+
+def tensors():
+    """The compiled tensor-level calls (csrc/tensors.cpp); they need torch to be imported."""
+    global _tensors
+    if _tensors is None:
+        if not os.path.exists(TENSORS):
+            raise LibraryMissing(
+                f"{TENSORS} is missing: build it with `python -m batch_topk_b200.build`"
+            )
+        from . import _tensors as module
+
+        _tensors = module
+    return _tensors
 
 
 def load() -> C.CDLL:

@@ -1,4 +1,5 @@
-"""Builds the sm_100a shared library (batch_topk_b200/lib/libbatch_topk_b200.so) with nvcc.
+"""Builds the sm_100a shared library (batch_topk_b200/lib/libbatch_topk_b200.so) with nvcc, and the
+tensor-level Python module over it (batch_topk_b200/_tensors.so) with g++.
 
 Run as ``python -m batch_topk_b200.build``.  The library is built in-tree so that it
 travels with the repository; nothing is installed into site-packages.
@@ -27,6 +28,8 @@ HEADERS = [os.path.join(HERE, "csrc", f) for f in ("bt_device.cuh", "bt_kernels.
 SOURCES = [SRC, GEN_SRC, LOGITS_SRC, SAMPLE_SRC, EXPERTS_SRC]
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libbatch_topk_b200.so")
+TENSORS_SRC = os.path.join(HERE, "csrc", "tensors.cpp")  # needs torch's headers
+TENSORS = os.path.join(HERE, "_tensors.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -49,20 +52,54 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(p) <= t for p in [*SOURCES, *HEADERS])
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and up_to_date():
-        return LIB
-    os.makedirs(LIB_DIR, exist_ok=True)
-    tmp = LIB + ".tmp"
-    cmd = [nvcc(), *NVCC_FLAGS, "--threads", "0", "-o", tmp, *SOURCES]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
+def tensors_up_to_date() -> bool:
+    if not os.path.exists(TENSORS):
+        return False
+    t = os.path.getmtime(TENSORS)
+    return all(os.path.getmtime(p) <= t for p in [TENSORS_SRC, *HEADERS])
+
+
+def _run(cmd: list[str], verbose: bool = False) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        raise RuntimeError(f"{cmd[0]} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
     if verbose:
         sys.stderr.write(res.stderr)
-    os.replace(tmp, LIB)
+
+
+def build_tensors(force: bool = False) -> str:
+    """The Python module; LIB has to be there (it is linked, and found beside the module)."""
+    if not force and tensors_up_to_date():
+        return TENSORS
+    import sysconfig
+    from importlib.util import find_spec
+
+    torch_dir = os.path.dirname(find_spec("torch").origin)
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    tmp = TENSORS + ".tmp"
+    # the g++ that nvcc compiles host code with: another one may bring its own C++ library
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+          "-D_GLIBCXX_USE_CXX11_ABI=1",
+          "-I" + os.path.join(torch_dir, "include"),
+          "-I" + os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+          "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda, "include"),
+          TENSORS_SRC, "-o", tmp,
+          "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+          "-ltorch_python", "-L" + LIB_DIR, "-lbatch_topk_b200", "-Wl,-rpath,$ORIGIN/lib"])
+    os.replace(tmp, TENSORS)
+    return TENSORS
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    if force or not up_to_date():
+        os.makedirs(LIB_DIR, exist_ok=True)
+        tmp = LIB + ".tmp"
+        cmd = [nvcc(), *NVCC_FLAGS, "--threads", "0", "-o", tmp, *SOURCES]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+        _run(cmd, verbose)
+        os.replace(tmp, LIB)
+    build_tensors(force)
     return LIB
 
 
