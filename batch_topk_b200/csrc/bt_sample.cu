@@ -212,9 +212,16 @@ struct Slice {
   const uint4* base;
   int shift, vocab, vecs, v0, v1, i0, i1;
 
-  __device__ __forceinline__ uint4 raw(int v) const {
-    return v < v1 ? __ldg(base + v) : V::neg_inf();
+  // Rows stream past the L1 cache, which keeps the threads' local variables (with the rows in it, a
+  // block took twice as long).
+  __device__ __forceinline__ uint4 stream(int v) const {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(base + v));
+    return r;
   }
+  __device__ __forceinline__ uint4 raw(int v) const { return v < v1 ? stream(v) : V::neg_inf(); }
   // Vector v of the slice from its bytes: nothing from outside the row.
   __device__ __forceinline__ uint4 fix(int v, uint4 r) const {
     if (v == 0 || v == vecs - 1) {
@@ -388,8 +395,8 @@ struct Sampler {
   static constexpr int kPer = S::kPer;
   static constexpr bool kBf16 = sizeof(typename E::T) == 2 && V::kBf16;
 
-  const Params& p;
-  Team& team;
+  const Params& p;  // the kernel's, which stays in constant memory
+  Team team;
   Shared& sh;
   S s;
   float* slot;          // [slots][kThreads] group maxima
@@ -540,7 +547,7 @@ struct Sampler {
   struct Stat {
     float top, sum;
   };
-  static __device__ __noinline__ Stat scan(const S s, float c, float* slot, int slots,
+  static __device__ __forceinline__ Stat scan(const S s, float c, float* slot, int slots,
                                            int groups_per_slot) {
     Running w;
     if (threadIdx.x < 2) {  // the row's first and last vectors
@@ -557,7 +564,7 @@ struct Sampler {
 #pragma unroll
     for (int u = 0; u < kGroup; ++u) {
       r[u] = V::neg_inf();
-      if (first + u * kThreads < s.i1) r[u] = __ldg(s.base + first + u * kThreads);
+      if (first + u * kThreads < s.i1) r[u] = s.stream(first + u * kThreads);
     }
     int whole = (s.i1 - s.i0) / stride;  // groups that every thread has in full
     for (int at = 0; at < slots; ++at) {
@@ -576,7 +583,7 @@ struct Sampler {
         first += stride;
 #pragma unroll
         for (int u = 0; u < kGroup; ++u) {
-          if (first + u * kThreads < s.i1) r[u] = __ldg(s.base + first + u * kThreads);
+          if (first + u * kThreads < s.i1) r[u] = s.stream(first + u * kThreads);
         }
         const float most = fmaxf(V::max2(now[0], now[1]), V::max2(now[2], now[3]));
         top = fmaxf(top, most);
@@ -1206,7 +1213,7 @@ struct Sampler {
 };
 
 template <class E>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(Params p) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) unsigned char smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
   Team team{cg::this_cluster(), sh, 1, 0};
@@ -1286,7 +1293,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(Params p
     mass = 0.0f;
     if (n > kCap || few) {
       const int from = by_k ? last : lowest;
-      Sampler<E> slow = k;  // the rare functions stay out of line, and k in registers
+      // the rare functions stay out of line and work on a copy, so that k stays in registers
+      Sampler<E> slow = k;
       slow.weigh(by_k, from, 0, 0.0f);
       int at = sh.bin, end = sh.bin_end;
       above = sh.above;
@@ -1306,7 +1314,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(Params p
         k.open_list();
         float got;
         n = k.gather(end, &got);
-        passes = n > kCap || (!by_k && end < lowest && got < k.top_p * k.z * 1.00001f);
+        passes = n > kCap || (!by_k && end < lowest && got < k.top_p * k.z * 1.000002f);
       } else if (end < kBins && inside <= kCap && !(by_k && by_p)) {
         Sum up;
         double in;
@@ -1314,6 +1322,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(Params p
         mass = static_cast<float>(up.mass);
         // the cut has to lie in these bins by the exact weights too
         passes = by_p && !(mass < k.top_p * k.z && up.mass + in >= k.top_p * k.z);
+        k.team.parity = slow.team.parity;
       } else {
         passes = true;
       }
@@ -1327,8 +1336,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(Params p
         best = over > best ? over : best;
         // every quotient 0 or none: an element of weight 0, beyond the list, may win
         if (__syncthreads_or(threadIdx.x == 0 && (best >> 32) <= value_key(0.0f))) {
-          team.blocks = 1;
           Sampler<E> slow = k;
+          slow.team.blocks = 1;
           slow.s.v0 = 0;
           slow.s.v1 = slow.s.vecs;
           best = slow.by_passes(&total);
@@ -1357,7 +1366,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(Params p
         }
       });
     }
-    best = team.best(best);
+    best = k.team.best(best);
     passes = open_race && (best >> 32) <= value_key(0.0f);  // every quotient 0 or none
   }
   if (passes) {
