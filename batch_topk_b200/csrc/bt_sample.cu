@@ -46,7 +46,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kBlocksPerSm = 4;
+constexpr int kBlocksPerSm = 3;
 constexpr int kGroup = 4;         // vectors a thread loads at a time
 constexpr int kMaxSlots = 20;     // group maxima a thread keeps
 constexpr int kCap = 1024;        // list entries
@@ -289,7 +289,7 @@ struct Shared {
   uint32_t runs[kThreads];  // kth_bin's counts
   union {
     uint16_t hot[kMaxHot];  // groups to read again: slot * kThreads + thread
-    uint32_t place[256];
+    uint32_t place[kThreads];
   };
   float2 warp_stat[kWarps];
   float2 block_stat[kMaxCluster];
@@ -411,6 +411,23 @@ struct Sampler {
     return x == m ? 0.0f : __fmul_rn(__fsub_rn(x, m), inv);
   }
   __device__ __forceinline__ float weight(float x) const { return expf(scaled(x)); }
+
+  // A thread's race: quotients in approximate weights pass over elements that cannot win (the
+  // approximation is within 1e-5 of the weight), the others are compared exactly.
+  struct Race {
+    float lead = 0.0f;
+    u64 best = 0;
+  };
+  __device__ __forceinline__ float weight_near(float x) const {
+    return exp2_approx(x == m ? 0.0f : (x - m) * c);
+  }
+  __device__ __forceinline__ void race(Race& w, float x, int i, float near) const {
+    const float q = __ldg(noise + i);
+    if (near < 0.9999f * w.lead * q) return;
+    w.lead = fmaxf(w.lead, __fdividef(near, q));
+    const u64 e = entry(x, i);
+    w.best = e > w.best ? e : w.best;
+  }
 
   // The race's number: ordered quotient, then the lower index; every kept element's is above 0.
   __device__ __forceinline__ u64 entry(float x, int i) const {
@@ -923,7 +940,7 @@ struct Sampler {
   // Ranks n <= kCap entries (of sh.list, or in place) into sh.sorted, best first, and sets
   // sh.score to the entries' weights and noise.
   __device__ __forceinline__ void rank_list(const u64* list, uint32_t n) {
-    if (n <= 256) {  // each entry's place is the number of entries before it
+    if (n <= kThreads) {  // each entry's place is the number of entries before it
       uint32_t width = 32;
       while (width < n) width *= 2;
       const uint32_t mine = threadIdx.x & (width - 1), part = threadIdx.x / width;
@@ -950,7 +967,7 @@ struct Sampler {
       __syncthreads();
       return;
     }
-    uint32_t width = 512;
+    uint32_t width = kThreads;
     while (width < n) width *= 2;
     for (uint32_t i = threadIdx.x; i < width; i += kThreads) {
       sh.sorted[i] = i < n ? list[i] : ~0ull;
@@ -1073,13 +1090,13 @@ struct Sampler {
     open_list();
     float za = 0.0f, zi = 0.0f;
     uint32_t n = 0;
-    u64 top = 0;
+    Race run;
     const float low = bin_floor(fine_of < 0 ? end : fine_end);
     s.each([&](float x) { return x >= low; }, [&](int i, float x) {
       if (!(x >= low)) return;
       const int b = fine_bin(x);
       if (b > end) return;
-      const float w = weight(x);
+      const float w = weight_near(x);
       if (b >= at) {
         zi += w;
         const uint32_t to = atomicAdd(&sh.count, 1u);
@@ -1087,17 +1104,14 @@ struct Sampler {
       } else {
         za += w;
         ++n;
-        if (!(w < min_p)) {
-          const u64 e = entry(x, i);
-          top = e > top ? e : top;
-        }
+        if (!(min_p > 0.0f) || !(weight(x) < min_p)) race(run, x, i, w);
       }
     });
     float unused;
     const uint32_t listed = close_list(0.0f, &unused);
     *above = team.sum(za, n);
     *inside = team.sum(zi, 0).mass;
-    *best = team.best(top);
+    *best = team.best(run.best);
     return listed;
   }
 
@@ -1193,14 +1207,13 @@ struct Sampler {
         last = hi;
       }
     }
-    u64 best = 0;
+    Race run;
     s.each([&](int i, float x) {
       if (x > kNegInf && (x > cut || (x == cut && i <= last)) && !(weight(x) < min_p)) {
-        const u64 e = entry(x, i);
-        best = e > best ? e : best;
+        race(run, x, i, weight_near(x));
       }
     });
-    return team.best(best);
+    return team.best(run.best);
   }
 
   __device__ __forceinline__ void write(u64 best, float total, long long r) const {
@@ -1359,12 +1372,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(const __
       // the exponent's rounding is far below 1e-4 wherever the weight is above 2^-100
       const float low = k.min_p > 1e-30f ? k.m + (log2f(k.min_p) - 1e-4f) / k.c - fabsf(k.m) * 1e-6f
                                          : kNegInf;
+      typename Sampler<E>::Race run;
       k.each_hot(low, [&](int i, float x, bool) {
         if (x >= low && x > kNegInf && !(k.weight(x) < k.min_p)) {
-          const u64 e = k.entry(x, i);
-          best = e > best ? e : best;
+          k.race(run, x, i, k.weight_near(x));
         }
       });
+      best = run.best;
     }
     best = k.team.best(best);
     passes = open_race && (best >> 32) <= value_key(0.0f);  // every quotient 0 or none
@@ -1412,11 +1426,12 @@ int launch(Params p, int blocks, cudaStream_t stream) {
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-// Blocks a row: as many as keep about two blocks on each of 148 SMs busy, but no more than leave
-// each thread a vector.
+// Blocks a row: as many as give each of 148 SMs two blocks, but no more than leave each thread a
+// vector.  More blocks finish a row sooner but pay for their exchanges: 200 rows of 151936 without
+// filters take 56, 41, 46 and 67 us with 1, 2, 4 and 8 blocks a row.
 int blocks_for(int rows, int vocab, int per) {
   int blocks = 1;
-  while (blocks < kMaxCluster && static_cast<long long>(rows) * blocks < 4 * 148 &&
+  while (blocks < kMaxCluster && static_cast<long long>(rows) * blocks < 2 * 148 &&
          static_cast<long long>(vocab) > static_cast<long long>(blocks) * kThreads * per) {
     blocks *= 2;
   }
