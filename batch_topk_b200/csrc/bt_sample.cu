@@ -998,7 +998,7 @@ struct Sampler {
   // the answer is the first warp's.
   __device__ __forceinline__ u64 finish(uint32_t n, bool by_k, uint32_t above, float mass) {
     const u64* list = sh.list;
-    if (n > 128) {
+    if (n > kThreads) {
       n = prune(n, by_k, above, mass);
       list = sh.sorted;
     }
@@ -1049,7 +1049,7 @@ struct Sampler {
   // Pass 2 of an overflowing row: counts and weights by bin of the elements of the bins up to
   // `last`, joined in every block; then sh.bin is the bin that holds the cut.
   // `above` elements of weight `heavier` lie before the bins that are looked through.
-  __device__ __noinline__ void weigh(bool by_k, int last, uint32_t above, float heavier) {
+  __device__ __forceinline__ void weigh_in(bool by_k, int last, uint32_t above, float heavier) {
     const float units = fminf(32768.0f, 4.0e9f / static_cast<float>(p.vocab));
     clear_bins();
     __syncthreads();
@@ -1086,7 +1086,8 @@ struct Sampler {
 
   // Pass 3: the elements of the bins [at, end] into the list; those above them are all kept, so
   // they are counted, summed and raced.  `inside`: the weight in the bins.
-  __device__ __noinline__ uint32_t split(int at, int end, Sum* above, double* inside, u64* best) {
+  __device__ __forceinline__ uint32_t split_in(int at, int end, Sum* above, double* inside,
+                                                u64* best) {
     open_list();
     float za = 0.0f, zi = 0.0f;
     uint32_t n = 0;
@@ -1125,7 +1126,7 @@ struct Sampler {
   }
 
   // Whole passes: the cut in rank order by bisection, then the race over what is above it.
-  __device__ __noinline__ u64 by_passes(float* total) {
+  __device__ __forceinline__ u64 by_passes_in(float* total) {
     float zt = 0.0f;
     uint32_t n = 0;
     s.each([&](int, float x) {
@@ -1214,6 +1215,32 @@ struct Sampler {
       }
     });
     return team.best(run.best);
+  }
+
+  // The rare passes out of line, each on a copy of its own: its members are then registers, where
+  // through `this` every element would load them again (20 us a pass instead of 5).
+  __device__ __noinline__ void weigh(bool by_k, int last, uint32_t above, float heavier) const {
+    Sampler me(*this);
+    me.weigh_in(by_k, last, above, heavier);
+  }
+  __device__ __noinline__ uint32_t split(int at, int end, Sum* above, double* inside, u64* best) {
+    Sampler me(*this);
+    Sum a;
+    double w;
+    u64 b;
+    const uint32_t n = me.split_in(at, end, &a, &w, &b);
+    *above = a;
+    *inside = w;
+    *best = b;
+    team.parity = me.team.parity;
+    return n;
+  }
+  __device__ __noinline__ u64 by_passes(float* total) const {
+    Sampler me(*this);
+    float t;
+    const u64 best = me.by_passes_in(&t);
+    *total = t;
+    return best;
   }
 
   __device__ __forceinline__ void write(u64 best, float total, long long r) const {
