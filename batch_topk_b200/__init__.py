@@ -168,7 +168,7 @@ def logits_topk_status(d_workspace: int, M: int, V: int, D: int, k: int, stream:
     return rc
 
 
-ELEM_F16, ELEM_BF16, ELEM_F32 = 0, 1, 2
+DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 MAX_EXPERTS = 1024
 MAX_EXPERTS_PER_TOKEN = 32

@@ -949,15 +949,15 @@ int route_of(const P& p, cudaStream_t s) {
 template <class F>
 int by_elem(int elem, F f) {
   switch (elem) {
-    case BT_ELEM_F16: return f(Elem<__half>{});
-    case BT_ELEM_BF16: return f(Elem<__nv_bfloat16>{});
-    case BT_ELEM_F32: return f(Elem<float>{});
+    case BT_DTYPE_F16: return f(Elem<__half>{});
+    case BT_DTYPE_BF16: return f(Elem<__nv_bfloat16>{});
+    case BT_DTYPE_F32: return f(Elem<float>{});
     default: return cudaErrorInvalidValue;
   }
 }
 
-size_t elem_size(int elem) { return elem == BT_ELEM_F32 ? 4 : 2; }
-bool elem_ok(int elem) { return elem == BT_ELEM_F16 || elem == BT_ELEM_BF16 || elem == BT_ELEM_F32; }
+size_t elem_size(int elem) { return elem == BT_DTYPE_F32 ? 4 : 2; }
+bool elem_ok(int elem) { return elem == BT_DTYPE_F16 || elem == BT_DTYPE_BF16 || elem == BT_DTYPE_F32; }
 
 // Threads over a row's vectors, a power of two, and rows side by side to fill the block.
 dim3 row_block(int nvec) {

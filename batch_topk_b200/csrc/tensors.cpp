@@ -84,9 +84,9 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
 
 int elem_of(const at::Tensor& t) {
   switch (t.scalar_type()) {
-    case at::kHalf: return BT_ELEM_F16;
-    case at::kBFloat16: return BT_ELEM_BF16;
-    case at::kFloat: return BT_ELEM_F32;
+    case at::kHalf: return BT_DTYPE_F16;
+    case at::kBFloat16: return BT_DTYPE_BF16;
+    case at::kFloat: return BT_DTYPE_F32;
     default: return -1;
   }
 }

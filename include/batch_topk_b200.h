@@ -176,13 +176,13 @@ int bt_logits_topk_status(const void* d_workspace, int M, int V, int D, int k, v
 
 /* Operators of a language model built on selection; no reference counterpart (the reference
  * selects and stops, include/batch_topk.cuh:10-19).  Common to all of them: `elem` names the type
- * of the values (BT_ELEM_*), strides count elements between rows (the values of a row are
+ * of the values (BT_DTYPE_*), strides count elements between rows (the values of a row are
  * adjacent), pointers are aligned to their elements, a call is asynchronous on `stream` and
  * needs no workspace (but bt_expert_order), and cudaErrorInvalidValue answers a bad shape, a NULL or misaligned pointer or an
  * unknown constant before anything is launched. */
-#define BT_ELEM_F16 0
-#define BT_ELEM_BF16 1
-#define BT_ELEM_F32 2
+#define BT_DTYPE_F16 0
+#define BT_DTYPE_BF16 1
+#define BT_DTYPE_F32 2
 
 /* One token for each row of logits [rows, vocab], by temperature, top-k, top-p and min-p, from
  * given random numbers.  1 <= vocab <= BT_MAX_SEG_LEN.

@@ -296,6 +296,17 @@ def test_combine(dtype, tokens, k, num, width, shift):
 
 
 @pytest.mark.gpu
+def test_dispatch_offsets_beyond_32_bits():
+    """Rows more than 2^31 elements apart."""
+    big = torch.empty((3, 2**30 + 24), dtype=torch.bfloat16, device="cuda")
+    x = big[:, -64:]
+    x.copy_(rand(3, 64, seed=1, dtype="bf16"))
+    plan = api.expert_order(torch.tensor([[1, 0], [0, 2], [2, 1]], dtype=torch.int32,
+                                         device="cuda"), 3)
+    assert torch.equal(api.dispatch(x, plan), x[plan.order.long() // 2])
+
+
+@pytest.mark.gpu
 def test_rows_gradient_differences():
     """combine(dispatch(x)) is linear in x and in the weights: differences give the gradients up to
     the rounding of float32 sums (2^-20 of terms of size below 64)."""

@@ -77,6 +77,40 @@ def test_sizes_and_settings(dtype, n, v):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+@pytest.mark.parametrize("scale", [0.3, 3.0])
+def test_long_rows(dtype, scale):
+    x, q = inputs(1, 3000017, dtype, 5, scale)
+    for kw in (dict(), dict(top_k=100), dict(top_k=5000, temperature=0.5), dict(top_p=0.7),
+               dict(min_p=0.2), dict(temperature=0.0)):
+        tokens, logprobs = api.sample(x, q, **kw)
+        check(x, q, tokens, logprobs, **kw)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Rows more than 2^31 elements apart."""
+    big = torch.empty((3, 2**30 + 24), dtype=torch.bfloat16, device="cuda")
+    x, q = inputs(3, 2003, "bf16", 19)
+    view = big[:, -2003:]
+    view.copy_(x)
+    for kw in (dict(), dict(top_k=20, top_p=0.9)):
+        tokens, logprobs = api.sample(view, q, **kw)
+        check(x, q, tokens, logprobs, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [150, 300, 600])
+def test_many_rows(dtype, n):
+    """Batches that take one, two or more blocks a row."""
+    x, q = inputs(n, 6007, dtype, n, 3.0)
+    for kw in (dict(), dict(top_k=20), dict(top_p=0.9), dict(top_p=0.95, temperature=3.0)):
+        tokens, logprobs = api.sample(x, q, **kw)
+        check(x, q, tokens, logprobs, **kw)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale", [0.0, 0.05, 0.6, 30.0])
 def test_flat_and_peaked_rows(dtype, scale):
@@ -264,7 +298,7 @@ def test_host_tensors_are_refused():
 
 def test_abi_argument_errors():
     """Rejected on the host before any CUDA work."""
-    def call(x=FAKE, elem=bt.ELEM_F32, rows=2, vocab=10, xs=10, q=FAKE, qs=10, dt=0, dk=0,
+    def call(x=FAKE, elem=bt.DTYPE_F32, rows=2, vocab=10, xs=10, q=FAKE, qs=10, dt=0, dk=0,
              tok=FAKE, lp=FAKE):
         return bt.sample(x, elem, rows, vocab, xs, q, qs, 1.0, dt, 0, dk, 1.0, 0, 0.0, 0, tok, lp)
 
