@@ -219,3 +219,79 @@ def _topk_segmented_op(x: torch.Tensor, offsets: torch.Tensor, k: int) -> tuple[
 def _topk_segmented_op_fake(x: torch.Tensor, offsets: torch.Tensor, k: int):
     n = offsets.shape[0] - 1
     return (x.new_empty((n, k)), x.new_empty((n, k), dtype=torch.int32))
+
+
+# Sampling and the experts' operators likewise (numbers for sample's settings; no gradients here:
+# train through route, dispatch and combine above).
+
+def _need(ok: bool, what: str):
+    if not ok:
+        raise ValueError(what)
+
+
+@torch.library.custom_op("batch_topk_b200::sample", mutates_args=())
+def _sample_op(logits: torch.Tensor, noise: torch.Tensor, temperature: float = 1.0,
+               top_k: int = 0, top_p: float = 1.0,
+               min_p: float = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
+    return sample(logits, noise, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+
+
+@_sample_op.register_fake
+def _sample_op_fake(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    _need(logits.dim() == 2 and logits.dtype in _ENTRY,
+          "logits must be a 2-D float16, bfloat16 or float32 tensor")
+    n = logits.shape[0]
+    return (logits.new_empty((n,), dtype=torch.int32), logits.new_empty((n,), dtype=torch.float32))
+
+
+@torch.library.custom_op("batch_topk_b200::route", mutates_args=())
+def _route_op(logits: torch.Tensor, k: int, score: str = "softmax",
+              bias: torch.Tensor | None = None, groups: int = 1, topk_groups: int = 1,
+              renormalize: bool = True, scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    return route(logits, k, score=score, bias=bias, groups=groups, topk_groups=topk_groups,
+                 renormalize=renormalize, scale=scale)
+
+
+@_route_op.register_fake
+def _route_op_fake(logits, k, score="softmax", bias=None, groups=1, topk_groups=1,
+                   renormalize=True, scale=1.0):
+    _need(logits.dim() == 2 and logits.dtype in _ENTRY,
+          "logits must be a 2-D float16, bfloat16 or float32 tensor")
+    n = logits.shape[0]
+    return (logits.new_empty((n, k), dtype=torch.float32),
+            logits.new_empty((n, k), dtype=torch.int32))
+
+
+@torch.library.custom_op("batch_topk_b200::expert_order", mutates_args=())
+def _expert_order_op(experts: torch.Tensor,
+                     num_experts: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return tuple(expert_order(experts, num_experts))
+
+
+@_expert_order_op.register_fake
+def _expert_order_op_fake(experts, num_experts):
+    _need(experts.dim() == 2 and experts.dtype == torch.int32, "experts must be a 2-D int32 tensor")
+    return (experts.new_empty((num_experts + 1,)), experts.new_empty((experts.numel(),)),
+            experts.new_empty(experts.shape))
+
+
+@torch.library.custom_op("batch_topk_b200::dispatch", mutates_args=())
+def _dispatch_op(x: torch.Tensor, offsets: torch.Tensor, order: torch.Tensor,
+                 position: torch.Tensor) -> torch.Tensor:
+    return dispatch(x, ExpertOrder(offsets, order, position))
+
+
+@_dispatch_op.register_fake
+def _dispatch_op_fake(x, offsets, order, position):
+    return x.new_empty((order.shape[0], x.shape[1]))
+
+
+@torch.library.custom_op("batch_topk_b200::combine", mutates_args=())
+def _combine_op(rows: torch.Tensor, offsets: torch.Tensor, order: torch.Tensor,
+                position: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
+    return combine(rows, ExpertOrder(offsets, order, position), weights)
+
+
+@_combine_op.register_fake
+def _combine_op_fake(rows, offsets, order, position, weights):
+    return rows.new_empty((position.shape[0], rows.shape[1]))
