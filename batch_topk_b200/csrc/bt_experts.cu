@@ -9,6 +9,7 @@
 //
 // No kernel uses a floating-point atomic: every sum has one fixed order, so results do not
 // change from run to run.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -498,75 +499,92 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 8 ? 16 : 1) route_bac
 // ---- order by expert ---------------------------------------------------------------------------
 //
 // Stable counting sort.  The entries are cut into contiguous runs, one a block and, inside, one a
-// warp.  A first kernel counts each block's experts; the second sums those counts to the places
-// where its entries begin (over experts, then blocks, then warps), and ranks each warp's run 32
-// entries at a time: lanes with the same expert find each other by one ballot for each bit of its
-// number (the match instruction takes four times as long).  A block first places its entries in
-// shared memory, so that each expert's share leaves for memory in whole lines: single scattered
-// stores would cost a memory transaction for every entry.  Runs of more than kTile entries a block
-// go tile by tile, with the counts taken again for each tile.  Few entries take one block, which
-// counts for itself.
+// warp.  A first kernel counts each block's experts and, in clusters of eight blocks, sums them over
+// the blocks before, so that the second has to read one row of counts for each cluster instead of
+// one for each block (5.0 us of 15 at 524168 entries and 256 experts).  The second turns the sums
+// into the places where its entries begin (over experts, then blocks, then warps) and ranks each
+// warp's run 32 entries at a time: lanes with the same expert find each other by one ballot for each
+// bit of its number (the match instruction in their place made the kernel 10 us slower).  A block first
+// places its entries in shared memory, so that each expert's share leaves for memory in whole
+// lines: single scattered stores would cost a memory transaction for every entry.  A run longer than
+// shared memory holds goes tile by tile.  Few entries take one block, which counts for itself.
+//
+// 524168 entries of 256 experts (6.3 MB, 1 us of memory time) take 14.5 us, 256 entries 6.2 us.
+// What bounds it are its dependent steps: launch and count, sums over clusters, experts and warps,
+// ranks, write-out, about 2 us each.
 
 struct OrderParams {
   const int* experts;
   int* offsets;
   int* order;
   int* position;
-  uint32_t* counts;  // [blocks][num], where there is more than one block
+  uint32_t* before;  // [blocks][num]: counts of the cluster's blocks before this one
+  uint32_t* total;   // [clusters][num]; both only where there is more than one block
   int n, num;
-  int per_block;  // entries of a block, a multiple of 32 * kOrderWarps
+  int per_block;  // entries of a block
+  int tile;       // of those, as many as shared memory holds at a time
 };
 
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
-constexpr int kTile = 32768;
-constexpr int kOrderAhead = 4;  // loads a lane keeps in flight
+constexpr int kOrderAhead = 4;   // loads a lane keeps in flight
 constexpr int kOrderRun = 4096;  // entries of a block, more where that would take over kOrderBlocks
-constexpr int kOrderBlocks = 256;
+constexpr int kOrderCluster = 8;
+// One wave: the kernel's registers leave room for one block an SM (two of 32 registers a thread are
+// no faster), and the clusters are whole.  256 blocks took 24.7 us instead of 18.5 us at 1048576
+// entries of 256 experts.
+constexpr int kOrderBlocks = 144;
+constexpr int kOrderSmem = 227 * 1024;
 
-// Calls f(entry, expert, whether there is one) for the run [a0, a1), 32 entries at a time in order,
-// with every lane; the expert is -1 outside [0, num).
-template <class F>
-__device__ __forceinline__ void each_entry(const OrderParams& p, int a0, int a1, F f) {
-  const int lane = threadIdx.x & 31;
-  for (int a = a0; a < a1; a += 32 * kOrderAhead) {
-    int e[kOrderAhead];
+// The experts of entries a + u * step for u < kOrderAhead, -1 where there is none.
+__device__ __forceinline__ void load_experts(const OrderParams& p, int a, int step, int end,
+                                             int (&e)[kOrderAhead]) {
 #pragma unroll
-    for (int u = 0; u < kOrderAhead; ++u) {
-      const int at = a + u * 32 + lane;
-      e[u] = at < a1 ? __ldg(p.experts + at) : -1;
-      if (static_cast<unsigned>(e[u]) >= static_cast<unsigned>(p.num)) e[u] = -1;
-    }
-#pragma unroll
-    for (int u = 0; u < kOrderAhead; ++u) {
-      if (a + u * 32 < a1) f(a + u * 32 + lane, e[u], a + u * 32 + lane < a1);
-    }
+  for (int u = 0; u < kOrderAhead; ++u) {
+    const int at = a + u * step;
+    e[u] = at < end ? __ldg(p.experts + at) : -1;
+    if (static_cast<unsigned>(e[u]) >= static_cast<unsigned>(p.num)) e[u] = -1;
   }
 }
 
-__global__ void __launch_bounds__(kOrderThreads) order_count_kernel(OrderParams p) {
+// The run of this block; the last ones can be empty.
+__device__ __forceinline__ void order_run(const OrderParams& p, int* first, int* last) {
+  const long long b0 = static_cast<long long>(blockIdx.x) * p.per_block;
+  *first = static_cast<int>(b0 < p.n ? b0 : p.n);
+  *last = static_cast<int>(b0 + p.per_block < p.n ? b0 + p.per_block : p.n);
+}
+
+__global__ void __cluster_dims__(kOrderCluster, 1, 1) __launch_bounds__(kOrderThreads)
+    order_count_kernel(OrderParams p) {
   extern __shared__ uint32_t smem[];
+  const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
   for (int e = threadIdx.x; e < p.num; e += kOrderThreads) smem[e] = 0;
   __syncthreads();
   bt::grid_dep_launch();
-  const long long b0 = static_cast<long long>(blockIdx.x) * p.per_block;
-  const int last = static_cast<int>(b0 + p.per_block < p.n ? b0 + p.per_block : p.n);
-  for (int a = static_cast<int>(b0) + threadIdx.x; a < last; a += kOrderThreads * kOrderAhead) {
+  int first, last;
+  order_run(p, &first, &last);
+  for (int a = first + threadIdx.x; a < last; a += kOrderThreads * kOrderAhead) {
     int e[kOrderAhead];
+    load_experts(p, a, kOrderThreads, last, e);
 #pragma unroll
     for (int u = 0; u < kOrderAhead; ++u) {
-      const int at = a + u * kOrderThreads;
-      e[u] = at < last ? __ldg(p.experts + at) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < kOrderAhead; ++u) {
-      if (static_cast<unsigned>(e[u]) < static_cast<unsigned>(p.num)) atomicAdd(&smem[e[u]], 1u);
+      if (e[u] >= 0) atomicAdd(&smem[e[u]], 1u);
     }
   }
-  __syncthreads();
+  cluster.sync();
+  const int rank = static_cast<int>(cluster.block_rank());
   for (int e = threadIdx.x; e < p.num; e += kOrderThreads) {
-    p.counts[static_cast<size_t>(blockIdx.x) * p.num + e] = smem[e];
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int r = 0; r < kOrderCluster; ++r) {
+      const uint32_t c = cluster.map_shared_rank(smem, r)[e];
+      before += r < rank ? c : 0u;
+      all += c;
+    }
+    p.before[static_cast<size_t>(blockIdx.x) * p.num + e] = before;
+    if (rank == 0) p.total[static_cast<size_t>(blockIdx.x / kOrderCluster) * p.num + e] = all;
   }
+  cluster.sync();
 }
 
 __global__ void __launch_bounds__(kOrderThreads) order_kernel(OrderParams p) {
@@ -575,157 +593,163 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(OrderParams p) {
   uint32_t* tot = cnt + kOrderWarps * p.num;  // [num]: the tile's counts
   uint32_t* base = tot + p.num;               // [num]: where this block's next entries go
   uint32_t* begin = base + p.num;             // [num]: where the tile's entries begin in `tile`
-  uint32_t* part = begin + p.num;             // [32]
-  uint16_t* tile = reinterpret_cast<uint16_t*>(part + 32);  // entries by expert
+  uint32_t* part = begin + p.num;             // [2][32]
+  uint32_t* tile = part + 64;                 // by expert: its number << 16 | place in the tile
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rank = blockIdx.x, blocks = gridDim.x;
-  const long long b0 = static_cast<long long>(rank) * p.per_block;
-  const int first = static_cast<int>(b0 < p.n ? b0 : p.n);
-  const int last = static_cast<int>(b0 + p.per_block < p.n ? b0 + p.per_block : p.n);
+  const int blocks = gridDim.x;
+  const bool owner = static_cast<int>(threadIdx.x) < p.num;  // of expert threadIdx.x
+  int first, last;
+  order_run(p, &first, &last);
   uint32_t* mine = cnt + warp * p.num;
+  const int bits = 32 - __clz(p.num - 1 > 0 ? p.num - 1 : 1);  // of an expert's number
+  uint32_t live = 0;
 
-  auto clear = [&]() {
+  for (int t0 = first;; t0 += p.tile) {
+    const int t1 = min(t0 + p.tile, last);
+    // this warp's share of the tile
+    const int per = (t1 - t0 + 32 * kOrderWarps - 1) / (32 * kOrderWarps) * 32;
+    const int a0 = min(t0 + warp * per, t1), a1 = min(a0 + per, t1);
     for (int i = threadIdx.x; i < kOrderWarps * p.num; i += kOrderThreads) cnt[i] = 0;
     __syncthreads();
-  };
-  auto count = [&](int a0, int a1) {
-    each_entry(p, a0, a1, [&](int, int e, bool) {
-      if (e >= 0) atomicAdd(&mine[e], 1u);
-    });
-    __syncthreads();
-  };
-  // per-warp counts to starts within the expert; their sum to tot
-  auto starts = [&]() {
-    for (int e = threadIdx.x; e < p.num; e += kOrderThreads) {
-      uint32_t run = 0;
-      for (int w = 0; w < kOrderWarps; ++w) {
-        const uint32_t c = cnt[w * p.num + e];
-        cnt[w * p.num + e] = run;
-        run += c;
-      }
-      tot[e] = run;
-    }
-    __syncthreads();
-  };
-  // exclusive sum over the threads (num <= threads); total in *all
-  auto scan = [&](uint32_t v, uint32_t* all) {
-    uint32_t incl = v;
+    for (int a = a0 + lane; a < a1; a += 32 * kOrderAhead) {
+      int e[kOrderAhead];
+      load_experts(p, a, 32, a1, e);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(kAll, incl, o);
-      if (lane >= o) incl += y;
-    }
-    __syncthreads();
-    if (lane == 31) part[warp] = incl;
-    __syncthreads();
-    uint32_t w = part[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(kAll, w, o);
-      if (lane >= o) w += y;
-    }
-    *all = __shfl_sync(kAll, w, 31);
-    const uint32_t pre = __shfl_sync(kAll, w, warp ? warp - 1 : 0);
-    return (warp ? pre : 0u) + incl - v;
-  };
-  auto run_of = [&](int t0, int t1, int* a0, int* a1) {  // this warp's share of a tile
-    const int per = (t1 - t0 + 32 * kOrderWarps - 1) / (32 * kOrderWarps) * 32;
-    *a0 = min(t0 + warp * per, t1);
-    *a1 = min(*a0 + per, t1);
-  };
-
-  const int bits = 32 - __clz(p.num - 1 > 0 ? p.num - 1 : 1);  // of an expert's number
-  const bool one_tile = p.per_block <= kTile;
-  int a0, a1;
-  run_of(first, last, &a0, &a1);
-  clear();
-  count(a0, a1);
-  starts();
-  uint32_t all = 0, before = 0;  // thread e: the count of expert e, and earlier blocks'
-  if (blocks == 1) {
-    if (threadIdx.x < p.num) all = tot[threadIdx.x];
-  } else {
-    // the blocks' counts, summed by as many threads an expert as there are
-    bt::grid_dep_wait();
-    int width = 32;
-    while (width < p.num) width *= 2;
-    const int e = threadIdx.x & (width - 1), shares = kOrderThreads / width;
-    if (threadIdx.x < p.num) base[threadIdx.x] = begin[threadIdx.x] = 0;
-    __syncthreads();
-    if (e < p.num) {
-      uint32_t a = 0, b = 0;
-#pragma unroll 8
-      for (int i = threadIdx.x / width; i < blocks; i += shares) {
-        const uint32_t c = __ldcg(p.counts + static_cast<size_t>(i) * p.num + e);
-        a += c;
-        b += i < rank ? c : 0u;
+      for (int u = 0; u < kOrderAhead; ++u) {
+        if (e[u] >= 0) atomicAdd(&mine[e[u]], 1u);
       }
-      atomicAdd(&base[e], a);  // base and begin hold the sums here
-      atomicAdd(&begin[e], b);
     }
     __syncthreads();
-    if (threadIdx.x < p.num) {
-      all = base[threadIdx.x];
-      before = begin[threadIdx.x];
-    }
-    __syncthreads();
-  }
-  uint32_t live;
-  const uint32_t at = scan(all, &live);
-  if (threadIdx.x < p.num) {
-    base[threadIdx.x] = at + before;
-    if (rank == 0) p.offsets[threadIdx.x] = static_cast<int>(at);
-  }
-  if (rank == 0 && threadIdx.x == 0) p.offsets[p.num] = static_cast<int>(live);
-
-  for (int t0 = first; t0 < last; t0 += kTile) {
-    const int t1 = min(t0 + kTile, last);
-    run_of(t0, t1, &a0, &a1);
-    if (!one_tile) {
-      __syncthreads();
-      clear();
-      count(a0, a1);
-      starts();
-    }
-    uint32_t in_tile;
-    const uint32_t from = scan(threadIdx.x < p.num ? tot[threadIdx.x] : 0u, &in_tile);
-    if (threadIdx.x < p.num) begin[threadIdx.x] = from;
-    __syncthreads();
-    each_entry(p, a0, a1, [&](int a, int e, bool in) {
-      unsigned peers = __ballot_sync(kAll, e >= 0);
+    // the warps' counts to starts within the expert
+    uint32_t count = 0;
+    if (owner) {
 #pragma unroll
-      for (int b = 0; b < 10; ++b) {
-        if (b >= bits) break;
-        const bool set = (e >> b) & 1;
-        const unsigned who = __ballot_sync(kAll, set);
-        peers &= set ? who : ~who;
-      }
-      const unsigned lower = peers & ((1u << lane) - 1u);
-      uint32_t start = 0;
-      if (e >= 0) start = mine[e];
-      __syncwarp();
-      if (e >= 0 && lower == 0) mine[e] = start + __popc(peers);
-      __syncwarp();
-      if (in) {
-        int pos = -1;
-        if (e >= 0) {
-          const uint32_t r = start + __popc(lower);
-          pos = static_cast<int>(base[e] + r);
-          tile[begin[e] + r] = static_cast<uint16_t>(a - t0);
+      for (int w0 = 0; w0 < kOrderWarps; w0 += 8) {
+        uint32_t c[8];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) c[w] = cnt[(w0 + w) * p.num + threadIdx.x];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          cnt[(w0 + w) * p.num + threadIdx.x] = count;
+          count += c[w];
         }
-        p.position[a] = pos;
       }
-    });
-    __syncthreads();
-    for (int e = warp; e < p.num; e += kOrderWarps) {
-      const uint32_t n = tot[e], src = begin[e], dst = base[e];
-      for (uint32_t i = lane; i < n; i += 32) p.order[dst + i] = t0 + tile[src + i];
-      __syncwarp();
-      if (lane == 0) base[e] = dst + n;
     }
+    uint32_t all = 0, before = 0;  // the expert's entries, and those of earlier blocks
+    if (t0 == first) {
+      if (blocks == 1) {
+        all = count;
+      } else {
+        // the clusters' counts, summed by as many threads an expert as there are
+        if (owner) base[threadIdx.x] = begin[threadIdx.x] = 0;
+        __syncthreads();
+        bt::grid_dep_wait();
+        int width = 32;
+        while (width < p.num) width *= 2;
+        const int e = threadIdx.x & (width - 1), shares = kOrderThreads / width;
+        const int mine_of = blockIdx.x / kOrderCluster;
+        const int clusters = (blocks + kOrderCluster - 1) / kOrderCluster;
+        if (e < p.num) {
+          uint32_t a = 0, b = 0;
+#pragma unroll 4
+          for (int i = threadIdx.x / width; i < clusters; i += shares) {
+            const uint32_t c = __ldcg(p.total + static_cast<size_t>(i) * p.num + e);
+            a += c;
+            b += i < mine_of ? c : 0u;
+          }
+          if (static_cast<int>(threadIdx.x) < width) {
+            b += __ldcg(p.before + static_cast<size_t>(blockIdx.x) * p.num + e);
+          }
+          atomicAdd(&base[e], a);  // base and begin hold the sums here
+          atomicAdd(&begin[e], b);
+        }
+        __syncthreads();
+        if (owner) {
+          all = base[threadIdx.x];
+          before = begin[threadIdx.x];
+        }
+      }
+    }
+    // exclusive sums over the experts (at most as many as threads)
+    uint32_t sum_all = all, sum_count = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(kAll, sum_all, o), y = __shfl_up_sync(kAll, sum_count, o);
+      if (lane >= o) {
+        sum_all += x;
+        sum_count += y;
+      }
+    }
+    if (lane == 31) {
+      part[warp] = sum_all;
+      part[32 + warp] = sum_count;
+    }
+    __syncthreads();
+    {
+      uint32_t x = part[lane], y = lane < warp ? part[32 + lane] : 0u;
+      if (t0 == first) live = __reduce_add_sync(kAll, x);
+      x = __reduce_add_sync(kAll, lane < warp ? x : 0u);
+      y = __reduce_add_sync(kAll, y);
+      sum_all += x - all;
+      sum_count += y - count;
+    }
+    if (owner) {
+      tot[threadIdx.x] = count;
+      begin[threadIdx.x] = sum_count;
+      if (t0 == first) {
+        base[threadIdx.x] = sum_all + before;
+        if (blockIdx.x == 0) p.offsets[threadIdx.x] = static_cast<int>(sum_all);
+      }
+    }
+    __syncthreads();
+    // ranks
+    for (int a = a0 + lane; a - lane < a1; a += 32 * kOrderAhead) {
+      int e[kOrderAhead];
+      load_experts(p, a, 32, a1, e);
+      unsigned peers[kOrderAhead];
+#pragma unroll
+      for (int u = 0; u < kOrderAhead; ++u) peers[u] = __ballot_sync(kAll, e[u] >= 0);
+      for (int b = 0; b < bits; ++b) {
+#pragma unroll
+        for (int u = 0; u < kOrderAhead; ++u) {
+          const bool set = (e[u] >> b) & 1;
+          const unsigned who = __ballot_sync(kAll, set);
+          peers[u] &= set ? who : ~who;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kOrderAhead; ++u) {
+        const int at = a + u * 32;
+        const unsigned lower = peers[u] & ((1u << lane) - 1u);
+        uint32_t start = 0;
+        if (e[u] >= 0) start = mine[e[u]];
+        __syncwarp();
+        if (e[u] >= 0 && lower == 0) mine[e[u]] = start + __popc(peers[u]);
+        __syncwarp();
+        if (at < a1) {
+          int pos = -1;
+          if (e[u] >= 0) {
+            const uint32_t r = start + __popc(lower);
+            pos = static_cast<int>(base[e[u]] + r);
+            tile[begin[e[u]] + r] = static_cast<uint32_t>(e[u]) << 16 | static_cast<uint32_t>(at - t0);
+          }
+          p.position[at] = pos;
+        }
+      }
+    }
+    __syncthreads();
+    const uint32_t in_tile = begin[p.num - 1] + tot[p.num - 1];
+    for (uint32_t i = threadIdx.x; i < in_tile; i += kOrderThreads) {
+      const uint32_t v = tile[i], e = v >> 16;
+      p.order[base[e] - begin[e] + i] = t0 + static_cast<int>(v & 0xFFFFu);
+    }
+    if (last - t0 <= p.tile) break;
+    __syncthreads();
+    if (owner) base[threadIdx.x] += count;
   }
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.offsets[p.num] = static_cast<int>(live);
   // places past the last live entry
-  for (long long i = static_cast<long long>(live) + rank * kOrderThreads + threadIdx.x; i < p.n;
+  for (long long i = static_cast<long long>(live) + blockIdx.x * kOrderThreads + threadIdx.x; i < p.n;
        i += static_cast<long long>(blocks) * kOrderThreads) {
     p.order[i] = -1;
   }
@@ -981,10 +1005,11 @@ bool wide(int elem, int width, long long stride, const void* a, const void* b, c
          aligned(c, 16);
 }
 
-size_t order_smem(int experts, long long per_block) {
-  const long long tile = per_block < kTile ? per_block : kTile;
-  return sizeof(uint32_t) * (kOrderWarps * experts + 3 * experts + 32) +
-         sizeof(uint16_t) * static_cast<size_t>(tile);
+// Shared memory of order_kernel beside its tile, and the tile that fits next to it.
+size_t order_fixed(int experts) { return sizeof(uint32_t) * (kOrderWarps * experts + 3 * experts + 64); }
+int order_tile(int experts, int per_block) {
+  const int room = static_cast<int>((kOrderSmem - order_fixed(experts)) / sizeof(uint32_t)) / 1024 * 1024;
+  return per_block < room ? per_block : room;
 }
 
 // Blocks, and a block's entries: one block while its threads take four entries each.
@@ -997,6 +1022,8 @@ int order_blocks(int n, int* per_block) {
   return static_cast<int>((n + per - 1) / per);
 }
 
+int order_clusters(int blocks) { return (blocks + kOrderCluster - 1) / kOrderCluster; }
+
 // Once per device: shared memory beyond the default.
 int order_ready() {
   static bool known[64] = {};
@@ -1007,7 +1034,7 @@ int order_ready() {
   std::lock_guard<std::mutex> lock(g_mu);
   if (!known[dev]) {
     e = cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(order_smem(BT_MAX_EXPERTS, kTile)));
+                             kOrderSmem);
     if (e != cudaSuccess) return e;
     known[dev] = true;
   }
@@ -1062,8 +1089,9 @@ int bt_route_backward(const void* d_logits, int elem, int tokens, int experts, l
 size_t bt_expert_order_workspace_size(int n, int experts) {
   if (n <= 0 || n > BT_MAX_ASSIGNMENTS || experts <= 0 || experts > BT_MAX_EXPERTS) return 0;
   int per = 0;
-  const int blocks = bte::order_blocks(n, &per);
-  return (sizeof(uint32_t) * static_cast<size_t>(blocks) * experts + 255) / 256 * 256;
+  const int blocks = bte::order_blocks(n, &per), clusters = bte::order_clusters(blocks);
+  return (sizeof(uint32_t) * static_cast<size_t>(clusters) * (bte::kOrderCluster + 1) * experts + 255) /
+         256 * 256;
 }
 
 int bt_expert_order(const int* d_experts, int n, int experts, int* d_offsets, int* d_order,
@@ -1077,21 +1105,23 @@ int bt_expert_order(const int* d_experts, int n, int experts, int* d_offsets, in
     return cudaErrorInvalidValue;
   }
   if (const int rc = order_ready()) return rc;
-  OrderParams p{d_experts, d_offsets, d_order, d_position, static_cast<uint32_t*>(d_workspace), n,
-                experts, 0};
-  const int blocks = order_blocks(n, &p.per_block);
+  OrderParams p{d_experts, d_offsets, d_order, d_position, nullptr, nullptr, n, experts, 0, 0};
+  const int blocks = order_blocks(n, &p.per_block), clusters = order_clusters(blocks);
+  p.tile = order_tile(experts, p.per_block);
+  p.before = static_cast<uint32_t*>(d_workspace);
+  p.total = p.before + static_cast<size_t>(clusters) * kOrderCluster * experts;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(kOrderThreads);
-  cfg.dynamicSmemBytes = order_smem(experts, p.per_block);
+  cfg.dynamicSmemBytes = order_fixed(experts) + sizeof(uint32_t) * p.tile;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   if (blocks > 1) {
     // the second kernel may start while the first runs, and waits for its counts
-    order_count_kernel<<<blocks, kOrderThreads, sizeof(uint32_t) * experts, s>>>(p);
+    order_count_kernel<<<clusters * kOrderCluster, kOrderThreads, sizeof(uint32_t) * experts, s>>>(p);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cfg.attrs = attr;
