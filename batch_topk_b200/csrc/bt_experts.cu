@@ -89,10 +89,14 @@ __device__ __forceinline__ float exp2_approx(float v) {
 // One warp a token; lane l owns the NPL experts from l * NPL, so a lower lane always holds lower
 // expert numbers and the first lane of a ballot resolves ties by index.
 //
-// The choice costs about one pass: the k-th largest of the lanes' maxima (a bitonic sort across
-// the warp) is a bound that at least k experts reach and few more (about 9 for k = 8 of 256).
-// Those go through shared memory to one lane each, and a lane's rank is the number of candidates
-// before its own.  More than 32 candidates (ties, or fewer than k open lanes) are taken one by one.
+// The choice costs about one pass: the k-th largest of the lanes' maxima is a bound that at least k
+// experts reach and few more (about 9 for k = 8 of 256).  Those go through shared memory to one lane
+// each, and a lane's rank is the number of candidates before its own.  More than 32 candidates (many
+// ties, or k near 32) are taken one by one.
+//
+// 131072 tokens of 256 fp32 logits, k = 8: 66 us forward, 52 us backward.  The forward kernel is
+// bound by its instructions (about 430 a token, of which 8 a lane are the row's own arithmetic), not
+// by its 134 MB; the backward kernel moves 5.4 TB/s.
 
 struct RouteParams {
   const void* logits;
@@ -106,6 +110,7 @@ struct RouteParams {
 };
 
 constexpr int kRouteWarps = 4;
+constexpr int kBoundSteps = 12;  // see kth_of_lanes
 
 // 1 / (1 + exp(-x)), each operation rounded once: the choice of experts compares these sums,
 // so no step may be contracted or approximated.
@@ -146,6 +151,19 @@ __device__ __forceinline__ float warp_sort_down(float v) {
     }
   }
   return __uint_as_float(bits);
+}
+
+// A value that at least k lanes reach, and few more: the k-th largest, or with a small k the k-th
+// largest of the different ones, which takes k short steps (131072 tokens of 256 experts, k = 8:
+// 66 us against 70 us with the sort, 12: 72 against 74; even at 16).
+__device__ __forceinline__ float kth_of_lanes(float v, int k) {
+  if (k > kBoundSteps) return __shfl_sync(kAll, warp_sort_down(v), k - 1);
+  float top = warp_max(v);
+  for (int j = 1; j < k; ++j) {
+    v = v == top ? kNegInf : v;
+    top = warp_max(v);
+  }
+  return top;
 }
 
 // The lane's logits: NaN reads as -inf, and so does every place past the last expert.  WIDE: the
@@ -324,8 +342,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) 
     }
   }
   // the bound, and who reaches it
-  const float sorted = warp_sort_down(row_max(c));
-  float bound = __shfl_sync(kAll, sorted, p.k - 1);
+  float bound = kth_of_lanes(row_max(c), p.k);
   if (near) bound -= 4e-6f + 1e-6f * fabsf(bound);
   bound = fmaxf(bound, -3.402823466e38f);  // closed experts are below every bound
   uint32_t mask = 0;  // this lane's candidates
@@ -759,7 +776,9 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(OrderParams p) {
 //
 // VEC elements a thread at a time: 16 bytes when the pointers, strides and width allow it, else one.
 // These kernels move bytes; what carries them is the number of independent loads in flight, so each
-// takes four rows at a time before the first is used.
+// takes four rows at a time before the first is used.  At 8191 tokens x 6 rows of 4 KB dispatch moves
+// 235 MB in 44 us, combine 235 MB in 43 us and its backward kernel 436 MB in 79 us: 5.3 to 5.5 TB/s,
+// 81 to 84% of a plain copy's rate.
 
 constexpr int kRowThreads = 256;
 constexpr int kAhead = 4;
@@ -990,7 +1009,7 @@ dim3 row_block(int nvec) {
   return dim3(x, kRowThreads / x);
 }
 // Blocks for `rows` rows, `per` of them a block: the scheduler evens them out over the SMs better
-// than a grid of resident blocks that stride over the rows (a sixth slower where 6 of 8 fit).
+// than a grid of resident blocks that stride over the rows.
 int row_grid(long long rows, int per) { return static_cast<int>((rows + per - 1) / per); }
 
 bool rows_ok(int tokens, int k, int width) {
