@@ -86,17 +86,17 @@ __device__ __forceinline__ float exp2_approx(float v) {
 
 // ---- routing ---------------------------------------------------------------------------------
 //
-// One warp a token; lane l owns the NPL experts from l * NPL, so a lower lane always holds lower
-// expert numbers and the first lane of a ballot resolves ties by index.
+// A warp, or half or a quarter of one, takes a token (see route_of); its lane l owns the NPL experts
+// from l * NPL, so a lower lane always holds lower expert numbers and the first lane of a ballot
+// resolves ties by index.
 //
 // The choice costs about one pass: the k-th largest of the lanes' maxima is a bound that at least k
-// experts reach and few more (about 9 for k = 8 of 256).  Those go through shared memory to one lane
-// each, and a lane's rank is the number of candidates before its own.  More than 32 candidates (many
-// ties, or k near 32) are taken one by one.
+// experts reach and few more (about 11 for k = 8 of 256).  Those go through shared memory to one lane
+// each, and a lane's rank is the number of candidates before its own.  More candidates than lanes
+// (many ties, or k near the lanes' number) are taken one by one.
 //
-// 131072 tokens of 256 fp32 logits, k = 8: 66 us forward, 52 us backward.  The forward kernel is
-// bound by its instructions (about 430 a token, of which 8 a lane are the row's own arithmetic), not
-// by its 134 MB; the backward kernel moves 5.4 TB/s.
+// 131072 tokens of 256 fp32 logits, k = 8: 53 us forward, 51 us backward (134 MB and 277 MB).  The
+// forward kernel is bound by its instructions and their latency, the backward kernel moves 5.4 TB/s.
 
 struct RouteParams {
   const void* logits;
@@ -122,26 +122,38 @@ __device__ __forceinline__ float sigmoid_near(float x) {
   return __fdividef(1.0f, 1.0f + exp2_approx(x * -kLog2e));
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
+// Over the L lanes of a token.
+template <int L = 32>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
   return v;
 }
-__device__ __forceinline__ float warp_max(float v) {  // no NaN
-  float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
+template <int L = 32>
+__device__ __forceinline__ float lanes_max(float v) {  // no NaN
+  if constexpr (L == 32) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+  } else {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
+    return v;
+  }
 }
 
-// Values of the warp sorted across its lanes, largest first.  Runs that have to be sorted the other
-// way hold negated values meanwhile, so that every exchange goes by one bit of the lane.
-__device__ __forceinline__ float warp_sort_down(float v) {
+// Values of L lanes sorted across them, largest first.  Runs that have to be sorted the other way
+// hold negated values meanwhile, so that every exchange goes by one bit of the lane.
+template <int L>
+__device__ __forceinline__ float lanes_sort_down(float v) {
+  constexpr int kLog = L == 32 ? 5 : (L == 16 ? 4 : 3);
+  static_assert(L == 1 << kLog, "8, 16 or 32 lanes");
   const uint32_t lane = threadIdx.x & 31;
   uint32_t bits = __float_as_uint(v);
 #pragma unroll
-  for (int log = 1; log <= 5; ++log) {
+  for (int log = 1; log <= kLog; ++log) {
     // negated in stage log: lanes with bit `log`; it was bit log - 1 in the stage before
-    const uint32_t flip = log == 1 ? lane >> 1 : (log == 5 ? lane >> 4 : (lane >> log) ^ (lane >> (log - 1)));
+    const uint32_t flip = log == 1 ? lane >> 1 : (log == kLog ? lane >> (log - 1) : (lane >> log) ^ (lane >> (log - 1)));
     bits ^= flip << 31;
 #pragma unroll
     for (int d = 1 << (log - 1); d > 0; d >>= 1) {
@@ -153,26 +165,27 @@ __device__ __forceinline__ float warp_sort_down(float v) {
   return __uint_as_float(bits);
 }
 
-// A value that at least k lanes reach, and few more: the k-th largest, or with a small k the k-th
-// largest of the different ones, which takes k short steps (131072 tokens of 256 experts, k = 8:
-// 66 us against 70 us with the sort, 12: 72 against 74; even at 16).
+// A value that at least k of L lanes reach, and few more: the k-th largest, or in a whole warp with a
+// small k the k-th largest of the different ones, which takes k short steps (131072 tokens of 256
+// experts, k = 8: 66 us against 70 us with the sort, 12: 72 against 74; even at 16).
+template <int L>
 __device__ __forceinline__ float kth_of_lanes(float v, int k) {
-  if (k > kBoundSteps) return __shfl_sync(kAll, warp_sort_down(v), k - 1);
-  float top = warp_max(v);
+  if (L < 32 || k > kBoundSteps) return __shfl_sync(kAll, lanes_sort_down<L>(v), k - 1, L);
+  float top = lanes_max<L>(v);
   for (int j = 1; j < k; ++j) {
     v = v == top ? kNegInf : v;
-    top = warp_max(v);
+    top = lanes_max<L>(v);
   }
   return top;
 }
 
 // The lane's logits: NaN reads as -inf, and so does every place past the last expert.  WIDE: the
 // rows are aligned for 16-byte loads and every lane's run is whole.
-template <class E, int NPL, bool WIDE>
+template <class E, int NPL, bool WIDE, int L = 32>
 __device__ __forceinline__ void load_logits(const typename E::T* row, int num, float (&x)[NPL]) {
   using T = typename E::T;
   constexpr int kPer = 16 / sizeof(T) < NPL ? 16 / sizeof(T) : NPL;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & (L - 1);
   if (WIDE) {
 #pragma unroll
     for (int i = 0; i < NPL; i += kPer) {
@@ -185,6 +198,26 @@ __device__ __forceinline__ void load_logits(const typename E::T* row, int num, f
     for (int i = 0; i < NPL; ++i) {
       const int e = lane * NPL + i;
       x[i] = e < num ? fmaxf(E::to_float(row[e]), kNegInf) : kNegInf;
+    }
+  }
+}
+
+template <int NPL, bool WIDE, int L>
+__device__ __forceinline__ void load_bias(const float* bias, int num, float (&b)[NPL]) {
+  constexpr int kPer = NPL < 4 ? NPL : 4;
+  const int lane = threadIdx.x & (L - 1);
+#pragma unroll
+  for (int i = 0; i < NPL; i += kPer) {
+    if (WIDE) {
+      const auto v = Pack<Elem<float>, kPer>::load(bias + lane * NPL + i);
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) b[i + q] = v.value(q);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        const int e = lane * NPL + i + q;
+        b[i + q] = e < num ? bias[e] : 0.0f;
+      }
     }
   }
 }
@@ -209,18 +242,18 @@ __device__ __forceinline__ float exp_near(float x, float m) {
 
 // The sum of the row's weights exp(x - m), from approximate exponentials.  Rows of +inf logits count
 // them; a row with nothing open gives 1e-30.
-template <int NPL>
+template <int NPL, int L = 32>
 __device__ __forceinline__ float row_sum(const float (&x)[NPL], float m) {
   float z = 0.0f;
   if (fabsf(m) < INFINITY) {
 #pragma unroll
     for (int i = 0; i < NPL; ++i) z += exp_near(x[i], m);
-    return warp_sum(z);
-  }
-  if (m == kNegInf) return 1e-30f;
+  } else {
 #pragma unroll
-  for (int i = 0; i < NPL; ++i) z += x[i] == m ? 1.0f : 0.0f;
-  return warp_sum(z);
+    for (int i = 0; i < NPL; ++i) z += x[i] == m ? 1.0f : 0.0f;
+  }
+  z = lanes_sum<L>(z);  // the lanes of a warp's other token take part
+  return m == kNegInf ? 1e-30f : z;
 }
 
 // Before in the choice: the larger value, equal values by lower index (-0 equals +0).
@@ -245,11 +278,17 @@ __device__ __forceinline__ void better_two(float& a, float& b, float oa, float o
   a = fmaxf(a, oa);
 }
 
-// Closes (sets to -inf) the choices of the groups that do not stay.
+// Floats from one lane's run to the next in shared memory: 16-byte accesses of eight lanes then
+// fall on different banks.
 template <int NPL>
+constexpr int kRunStride = NPL >= 8 ? NPL + 4 : NPL;
+
+// Closes (sets to -inf) the choices of the groups that do not stay.  L lanes hold at least as many
+// groups; `runs` is the token's shared memory.
+template <int NPL, int L>
 __device__ __forceinline__ void close_groups(const RouteParams& p, const float (&judged)[NPL],
-                                             float (&c)[NPL], float* shared) {
-  const int lane = threadIdx.x & 31, size = p.num / p.groups;
+                                             float (&c)[NPL], float* runs) {
+  const int lane = threadIdx.x & (L - 1), size = p.num / p.groups;
   float a = kNegInf, b = kNegInf;  // this lane's group's two best, or of group `lane`
   const int lanes = size / NPL;    // lanes a group covers, where it covers whole ones
   const bool whole = lanes * NPL == size && (lanes & (lanes - 1)) == 0 && lanes > 0;
@@ -262,10 +301,13 @@ __device__ __forceinline__ void close_groups(const RouteParams& p, const float (
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) shared[lane * NPL + i] = judged[i];
+    for (int i = 0; i < NPL; ++i) runs[lane * kRunStride<NPL> + i] = judged[i];
     __syncwarp();
     if (lane < p.groups) {
-      for (int i = 0; i < size; ++i) better_two(a, b, shared[lane * size + i], kNegInf);
+      for (int i = 0; i < size; ++i) {
+        const int e = lane * size + i;
+        better_two(a, b, runs[e / NPL * kRunStride<NPL> + e % NPL], kNegInf);
+      }
     }
     __syncwarp();
   }
@@ -275,7 +317,7 @@ __device__ __forceinline__ void close_groups(const RouteParams& p, const float (
   const int step = whole ? lanes : 1, mine = lane / step;
   int rank = 0;
   for (int g = 0; g < p.groups; ++g) {
-    const float o = __shfl_sync(kAll, score, g * step);
+    const float o = __shfl_sync(kAll, score, g * step, L);
     rank += before(o, g, score, mine);
   }
   const bool stays = mine < p.groups && rank < p.topk_groups;
@@ -283,7 +325,7 @@ __device__ __forceinline__ void close_groups(const RouteParams& p, const float (
 #pragma unroll
     for (int i = 0; i < NPL; ++i) c[i] = stays ? c[i] : kNegInf;
   } else {
-    const unsigned kept = __ballot_sync(kAll, stays);
+    const unsigned kept = __ballot_sync(kAll, stays) >> (threadIdx.x & 31 & ~(L - 1));
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
       const int e = lane * NPL + i;
@@ -292,20 +334,25 @@ __device__ __forceinline__ void close_groups(const RouteParams& p, const float (
   }
 }
 
-template <class E, int NPL, bool WIDE>
-__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) {
-  __shared__ __align__(16) unsigned long long found[kRouteWarps][32];  // candidates, see place_key
-  __shared__ __align__(16) float rows[kRouteWarps][32 * NPL];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + warp;
-  if (t >= p.tokens) return;
+template <class E, int NPL, bool WIDE, int L>
+__global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 16 ? 10 : 1) route_kernel(RouteParams p) {
+  constexpr int kStride = kRunStride<NPL>;
+  __shared__ __align__(16) unsigned long long slots[kRouteWarps * 32];  // candidates, see place_key
+  __shared__ __align__(16) float memory[kRouteWarps * 32 * kStride];
+  const int lane = threadIdx.x & (L - 1);  // of the token's
+  const int token = threadIdx.x / L;       // of the block's
+  const long long first = static_cast<long long>(blockIdx.x) * (kRouteWarps * 32 / L);
+  const bool live = first + token < p.tokens;  // the last warp's other token still takes part
+  const long long t = live ? first + token : p.tokens - 1;
+  unsigned long long* found = slots + token * L;
+  float* runs = memory + token * L * kStride;
   const auto* row = static_cast<const typename E::T*>(p.logits) + t * p.stride;
   float x[NPL];
-  load_logits<E, NPL, WIDE>(row, p.num, x);
+  load_logits<E, NPL, WIDE, L>(row, p.num, x);
   float m = 0.0f, z = 1.0f;
   if (!p.sigmoid) {
-    m = warp_max(row_max(x));
-    z = row_sum(x, m);
+    m = lanes_max<L>(row_max(x));
+    z = row_sum<NPL, L>(x, m);
   }
   // the score of one logit
   auto score_of = [&](float v) {
@@ -318,12 +365,12 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) 
 #pragma unroll
   for (int i = 0; i < NPL; ++i) c[i] = x[i];
   if (p.bias) {
+    float b[NPL];
+    load_bias<NPL, WIDE, L>(p.bias, p.num, b);
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
-      const int e = lane * NPL + i;
-      const float b = e < p.num ? p.bias[e] : 0.0f;
       const float s = near ? sigmoid_near(x[i]) : score_of(x[i]);
-      c[i] = x[i] == kNegInf ? kNegInf : fmaxf(__fadd_rn(s, b), kNegInf);
+      c[i] = x[i] == kNegInf ? kNegInf : fmaxf(__fadd_rn(s, b[i]), kNegInf);
     }
   }
   if (grouped) {
@@ -333,16 +380,16 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) 
       float s[NPL];
 #pragma unroll
       for (int i = 0; i < NPL; ++i) s[i] = x[i] == kNegInf ? kNegInf : sigmoid_rn(x[i]);
-      close_groups<NPL>(p, s, c, rows[warp]);
+      close_groups<NPL, L>(p, s, c, runs);
     } else {
       float judged[NPL];
 #pragma unroll
       for (int i = 0; i < NPL; ++i) judged[i] = c[i];
-      close_groups<NPL>(p, judged, c, rows[warp]);
+      close_groups<NPL, L>(p, judged, c, runs);
     }
   }
   // the bound, and who reaches it
-  float bound = kth_of_lanes(row_max(c), p.k);
+  float bound = kth_of_lanes<L>(row_max(c), p.k);
   if (near) bound -= 4e-6f + 1e-6f * fabsf(bound);
   bound = fmaxf(bound, -3.402823466e38f);  // closed experts are below every bound
   uint32_t mask = 0;  // this lane's candidates
@@ -351,27 +398,27 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) 
   const int own = __popc(mask);
   int at = own;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(kAll, at, o);
+  for (int o = 1; o < L; o <<= 1) {
+    const int y = __shfl_up_sync(kAll, at, o, L);
     if (lane >= o) at += y;
   }
-  const int n = __shfl_sync(kAll, at, 31);
+  const int n = __shfl_sync(kAll, at, L - 1, L);
   at -= own;
   int expert = -1;  // slot `lane`
-  if (n <= 32) {
-    found[warp][lane] = 0;  // behind every candidate
-    float* mine_of = rows[warp] + lane * NPL;  // indexed by a variable, which registers cannot be
+  if (!__any_sync(kAll, n > L)) {
+    found[lane] = 0;  // behind every candidate
+    float* run = runs + lane * kStride;  // indexed by a variable, which registers cannot be
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) mine_of[i] = c[i];
+    for (int i = 0; i < NPL; ++i) run[i] = c[i];
     __syncwarp();
     for (; mask; mask &= mask - 1) {
       const int i = __ffs(mask) - 1;
-      found[warp][at++] = place_key(mine_of[i], lane * NPL + i);
+      found[at++] = place_key(run[i], lane * NPL + i);
     }
     __syncwarp();
     unsigned long long mine = 0;
     if (lane < n) {
-      mine = found[warp][lane];
+      mine = found[lane];
       if (near) {  // now exactly
         const int e = place_expert(mine);
         mine = place_key(
@@ -380,21 +427,21 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) 
     }
     if (near) {
       __syncwarp();
-      if (lane < n) found[warp][lane] = mine;
+      if (lane < n) found[lane] = mine;
       __syncwarp();
     }
     int rank = 0;
     for (int j = 0; j < n; j += 4) {
 #pragma unroll
       for (int u = 0; u < 4; u += 2) {
-        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&found[warp][j + u]);
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&found[j + u]);
         rank += (two.x > mine) + (two.y > mine);
       }
     }
     __syncwarp();
-    if (lane < n) found[warp][rank] = mine;
+    if (lane < n) found[rank] = mine;
     __syncwarp();
-    if (lane < (n < p.k ? n : p.k)) expert = place_expert(found[warp][lane]);
+    if (lane < (n < p.k ? n : p.k)) expert = place_expert(found[lane]);
   } else {
     if (near) {
 #pragma unroll
@@ -403,27 +450,29 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteParams p) 
         if (c[i] > kNegInf) c[i] = __fadd_rn(sigmoid_rn(x[i]), p.bias[e]);
       }
     }
+    const int other = threadIdx.x & 31 & ~(L - 1);  // lanes before the token's
     for (int j = 0; j < p.k; ++j) {
       const float best = row_max(c);
-      const float top = warp_max(best);
-      if (top == kNegInf) break;  // nothing open is left
-      const int from = __ffs(__ballot_sync(kAll, best == top)) - 1;
-      int at = 0;
+      const float top = lanes_max<L>(best);
+      unsigned who = __ballot_sync(kAll, best == top) >> other;
+      if (L < 32) who &= (1u << (L & 31)) - 1u;
+      const int from = __ffs(who) - 1;
+      int place = 0;
 #pragma unroll
-      for (int i = NPL - 1; i >= 0; --i) at = c[i] == top ? i : at;
+      for (int i = NPL - 1; i >= 0; --i) place = c[i] == top ? i : place;
       if (lane == from) {
 #pragma unroll
-        for (int i = 0; i < NPL; ++i) c[i] = i == at ? kNegInf : c[i];
+        for (int i = 0; i < NPL; ++i) c[i] = i == place ? kNegInf : c[i];
       }
-      const int e = __shfl_sync(kAll, lane * NPL + at, from);
-      if (lane == j) expert = e;
+      const int e = __shfl_sync(kAll, lane * NPL + place, from, L);
+      if (lane == j && top > kNegInf) expert = e;  // else nothing open is left
     }
   }
   const float score =
       expert >= 0 ? score_of(fmaxf(E::to_float(row[expert]), kNegInf)) : 0.0f;
   float weight = p.scale * score;
-  if (p.renorm) weight /= warp_sum(score) + kRenormEps;
-  if (lane < p.k) {
+  if (p.renorm) weight /= lanes_sum<L>(score) + kRenormEps;
+  if (live && lane < p.k) {
     p.weights[t * p.k + lane] = weight;
     p.experts[t * p.k + lane] = expert;
   }
@@ -445,17 +494,19 @@ struct RouteBackParams {
 //   sigmoid: dx_j = ds_j s_j (1 - s_j) at the chosen experts, 0 elsewhere;
 //   softmax: dx_i = s_i (ds_i - sum_j ds_j s_j) everywhere.
 // Each lane writes its own run first; the chosen experts' values then replace theirs.
-template <class E, int NPL, bool WIDE>
-__global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 8 ? 16 : 1) route_backward_kernel(RouteBackParams p) {
+template <class E, int NPL, bool WIDE, int L>
+__global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 8 ? 16 : 1)
+    route_backward_kernel(RouteBackParams p) {
   using T = typename E::T;
   constexpr int kPer = 16 / sizeof(T) < NPL ? 16 / sizeof(T) : NPL;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + warp;
-  if (t >= p.tokens) return;
+  const int lane = threadIdx.x & (L - 1);  // of the token's
+  const long long at_token = static_cast<long long>(blockIdx.x) * (kRouteWarps * 32 / L) + threadIdx.x / L;
+  const bool live = at_token < p.tokens;  // the last warp's other tokens still take part
+  const long long t = live ? at_token : p.tokens - 1;
   const T* row = static_cast<const T*>(p.logits) + t * p.stride;
   T* out = static_cast<T*>(p.d_logits) + t * static_cast<long long>(p.num);
   float x[NPL], m = 0.0f, z = 1.0f, se, one_minus = 0.0f;
-  if (!p.sigmoid) load_logits<E, NPL, WIDE>(row, p.num, x);
+  if (!p.sigmoid) load_logits<E, NPL, WIDE, L>(row, p.num, x);
   int e = lane < p.k ? p.experts[t * p.k + lane] : -1;
   float g = lane < p.k ? p.scale * p.grad[t * p.k + lane] : 0.0f;
   if (e < 0 || e >= p.num) {
@@ -468,18 +519,18 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 8 ? 16 : 1) route_bac
     se = sigmoid_rn(xe);
     one_minus = xe > 0.0f ? u / (1.0f + u) : 1.0f / (1.0f + u);
   } else {
-    m = warp_max(row_max(x));
-    z = row_sum(x, m);
+    m = lanes_max<L>(row_max(x));
+    z = row_sum<NPL, L>(x, m);
     se = __fdiv_rn(exp_below(xe, m), z);
   }
   if (e < 0) se = 0.0f;
   float ds = g;
   if (p.renorm) {
-    const float total = warp_sum(se) + kRenormEps;
-    const float mean = warp_sum(g / total * se);  // a lane without an expert adds 0
+    const float total = lanes_sum<L>(se) + kRenormEps;
+    const float mean = lanes_sum<L>(g / total * se);  // a lane without an expert adds 0
     ds = e >= 0 ? g / total - mean / total : 0.0f;
   }
-  const float c = p.sigmoid ? 0.0f : warp_sum(ds * se);
+  const float c = p.sigmoid ? 0.0f : lanes_sum<L>(ds * se);
   float d[NPL];
   if (p.sigmoid || m == kNegInf) {
 #pragma unroll
@@ -492,7 +543,9 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 8 ? 16 : 1) route_bac
 #pragma unroll
     for (int i = 0; i < NPL; ++i) d[i] = x[i] == m ? -c / z : 0.0f;
   }
-  if (WIDE) {
+  if (!live) {
+    // nothing to write
+  } else if (WIDE) {
 #pragma unroll
     for (int i = 0; i < NPL; i += kPer) {
       Pack<E, kPer> v;
@@ -510,7 +563,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NPL <= 8 ? 16 : 1) route_bac
     }
   }
   __syncwarp();
-  if (e >= 0) out[e] = E::from_float(p.sigmoid ? ds * se * one_minus : se * (ds - c));
+  if (live && e >= 0) out[e] = E::from_float(p.sigmoid ? ds * se * one_minus : se * (ds - c));
 }
 
 // ---- order by expert ---------------------------------------------------------------------------
@@ -926,7 +979,7 @@ __global__ void __launch_bounds__(kRowThreads, 5)
       if (d_weights) {
 #pragma unroll
         for (int u = 0; u < kBackRows; ++u) {
-          dot[u] = warp_sum(dot[u]);
+          dot[u] = lanes_sum(dot[u]);
           if (lane == 0) part[warp][u] = dot[u];
         }
         __syncthreads();
@@ -957,36 +1010,67 @@ bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % 
 std::mutex g_mu;  // over what is looked up once per device
 
 // The kernel whose lanes own 1, 2, 4, 8, 16 or 32 experts each, wide where the rows allow it.
-template <class E, int NPL>
+template <class E, int NPL, int L>
 int launch_route(const RouteParams& p, cudaStream_t s) {
   using T = typename E::T;
   constexpr int kPer = 16 / sizeof(T) < NPL ? 16 / sizeof(T) : NPL;
-  const bool wide = p.num == 32 * NPL && p.stride % kPer == 0 && aligned(p.logits, sizeof(T) * kPer);
-  const int grid = (p.tokens + kRouteWarps - 1) / kRouteWarps;
-  if (wide) route_kernel<E, NPL, true><<<grid, 32 * kRouteWarps, 0, s>>>(p);
-  else route_kernel<E, NPL, false><<<grid, 32 * kRouteWarps, 0, s>>>(p);
+  constexpr int kTokens = kRouteWarps * 32 / L;
+  const bool wide = p.num == L * NPL && p.stride % kPer == 0 &&
+                    aligned(p.logits, sizeof(T) * kPer) && aligned(p.bias, 16);
+  const int grid = (p.tokens + kTokens - 1) / kTokens;
+  if (wide) route_kernel<E, NPL, true, L><<<grid, 32 * kRouteWarps, 0, s>>>(p);
+  else route_kernel<E, NPL, false, L><<<grid, 32 * kRouteWarps, 0, s>>>(p);
   return cudaGetLastError();
 }
-template <class E, int NPL>
+template <class E, int NPL, int L>
 int launch_route(const RouteBackParams& p, cudaStream_t s) {
   using T = typename E::T;
   constexpr int kPer = 16 / sizeof(T) < NPL ? 16 / sizeof(T) : NPL;
-  const bool wide = p.num == 32 * NPL && p.stride % kPer == 0 &&
+  constexpr int kTokens = kRouteWarps * 32 / L;
+  const bool wide = p.num == L * NPL && p.stride % kPer == 0 &&
                     aligned(p.logits, sizeof(T) * kPer) && aligned(p.d_logits, sizeof(T) * kPer);
-  const int grid = (p.tokens + kRouteWarps - 1) / kRouteWarps;
-  if (wide) route_backward_kernel<E, NPL, true><<<grid, 32 * kRouteWarps, 0, s>>>(p);
-  else route_backward_kernel<E, NPL, false><<<grid, 32 * kRouteWarps, 0, s>>>(p);
+  const int grid = (p.tokens + kTokens - 1) / kTokens;
+  if (wide) route_backward_kernel<E, NPL, true, L><<<grid, 32 * kRouteWarps, 0, s>>>(p);
+  else route_backward_kernel<E, NPL, false, L><<<grid, 32 * kRouteWarps, 0, s>>>(p);
   return cudaGetLastError();
 }
 
-template <class E, class P>
-int route_of(const P& p, cudaStream_t s) {
-  if (p.num <= 32) return launch_route<E, 1>(p, s);
-  if (p.num <= 64) return launch_route<E, 2>(p, s);
-  if (p.num <= 128) return launch_route<E, 4>(p, s);
-  if (p.num <= 256) return launch_route<E, 8>(p, s);
-  if (p.num <= 512) return launch_route<E, 16>(p, s);
-  return launch_route<E, 32>(p, s);
+template <class E, int L, class P>
+int route_with(const P& p, cudaStream_t s) {
+  if (p.num <= L) return launch_route<E, 1, L>(p, s);
+  if (p.num <= 2 * L) return launch_route<E, 2, L>(p, s);
+  if (p.num <= 4 * L) return launch_route<E, 4, L>(p, s);
+  if (p.num <= 8 * L) return launch_route<E, 8, L>(p, s);
+  if (L < 32 || p.num <= 16 * L) return launch_route<E, 16, L>(p, s);
+  if constexpr (L == 32) return launch_route<E, 32, L>(p, s);
+  return cudaErrorInvalidValue;
+}
+
+// Lanes a token.  What a token costs beside its experts (sums, sort, ranks) is paid once a warp, so
+// a warp takes as many tokens as leave a lane at most 16 experts, with twice as many lanes as
+// experts to choose: then few rows have more candidates than lanes.  131072 tokens with 32, 16 and 8
+// lanes: 256 experts, k = 8: 68 and 53 us; 128, k = 4: 49, 35 and 27 us; 8, k = 2: 39, 25 and 12 us.
+// With too few tokens to fill the SMs a whole warp is sooner done (4096 tokens of 256: 6.9 us
+// against 7.2 us).
+template <class E>
+int route_of(const RouteParams& p, cudaStream_t s) {
+  if (p.tokens / 32 >= p.num) {
+    if (p.k <= 4 && p.num <= 128 && p.groups <= 8) return route_with<E, 8>(p, s);
+    if (p.k <= 8 && p.num <= 256 && p.groups <= 16) return route_with<E, 16>(p, s);
+  }
+  return route_with<E, 32>(p, s);
+}
+// The backward kernel likewise, with a lane for each expert chosen and at most 32 bytes of the row a
+// lane: 131072 tokens, k = 8, with 32, 16 and 8 lanes: 128 bf16 experts 47, 31 and 21 us, 128 fp32
+// 49, 33 and 33 us; 256 fp32 experts 59 and 64 us, bf16 58 and 51 us.
+template <class E>
+int route_of(const RouteBackParams& p, cudaStream_t s) {
+  const size_t bytes = sizeof(typename E::T) * p.num;
+  if (p.tokens / 32 >= p.num) {
+    if (p.k <= 8 && bytes <= 8 * 32) return route_with<E, 8>(p, s);
+    if (p.k <= 16 && bytes <= 16 * 32) return route_with<E, 16>(p, s);
+  }
+  return route_with<E, 32>(p, s);
 }
 
 template <class F>
