@@ -114,6 +114,73 @@ def test_route_closed_experts(score, with_bias):
             assert (chosen[0] == -1).all() and (weights[0] == 0).all()
 
 
+MANY = [  # experts and settings; at least 32 tokens an expert, a warp takes several tokens
+    (5, dict(k=2)), (8, dict(k=4)), (8, dict(k=8)), (16, dict(k=8, score="sigmoid")),
+    (24, dict(k=3, score="sigmoid", bias=True)), (33, dict(k=5, renormalize=False)),
+    (40, dict(k=4, groups=8, topk_groups=5)), (60, dict(k=8, groups=12, topk_groups=9)),
+    (64, dict(k=6, score="sigmoid", groups=8, topk_groups=3, bias=True)),
+    (64, dict(k=8, groups=32, topk_groups=20)),
+    (96, dict(k=4, score="softmax", bias=True)), (128, dict(k=1, score="sigmoid", scale=0.5)),
+    (128, dict(k=4, score="sigmoid", groups=4, topk_groups=1)),
+    (200, dict(k=8, score="sigmoid", bias=True)), (256, dict(k=7)),
+    (256, dict(k=8, score="sigmoid", groups=8, topk_groups=4, bias=True, scale=2.5)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("experts,kw", MANY)
+def test_route_many_tokens(dtype, experts, kw):
+    """Ordinary rows next to rows of ties, closed experts and infinities, which need other paths
+    than their neighbours; every row like the same row in a small call."""
+    inf = float("inf")
+    kw = dict(kw)
+    if kw.get("bias"):
+        kw["bias"] = rand(experts, seed=experts, scale=0.1)
+    tokens = 32 * experts + 37
+    x = rand(tokens, experts, seed=experts, dtype=dtype, scale=1.5)
+    x[1::11] = x[1::11].round()
+    x[3::13] = 0.5
+    x[4::17, 1:] = -inf
+    x[5::19] = -inf
+    x[6::23, ::2] = float("nan")
+    x[7::29, 2] = inf
+    x[8::31, :3] = inf
+    x[9::37] = 200.0
+    weights, chosen = api.route(x, **kw)
+    rows = torch.cat([torch.arange(30), torch.arange(tokens - 10, tokens)]).cuda()
+    check_route(x[rows], weights[rows], chosen[rows], **kw)
+    for t in range(0, tokens, 32 * experts // 3):
+        part_w, part_e = api.route(x[t:t + 32], **kw)
+        assert torch.equal(chosen[t:t + 32], part_e)
+        # each within 2e-6 of the definition
+        assert (weights[t:t + 32] - part_w).abs().max() <= 4e-6 * kw.get("scale", 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("experts,k", [(5, 2), (8, 8), (40, 4), (64, 8), (100, 10), (128, 6),
+                                       (128, 16), (200, 9), (256, 8)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_gradient_many_tokens(dtype, experts, k, score):
+    tokens = 32 * experts + 5
+    x = rand(tokens, experts, seed=experts, dtype=dtype, scale=2.0)
+    x[0, 1] = float("-inf")
+    x[tokens - 2] = float("-inf")
+    x.requires_grad_()
+    weights, chosen = api.route(x, k, score=score, scale=2.0)
+    g = rand(tokens, k, seed=9)
+    dx, = torch.autograd.grad(weights, x, g)
+    xs, e, gs = x.detach().float().cpu().numpy(), chosen.cpu().numpy(), g.cpu().numpy()
+    for t in [*range(12), *range(tokens - 8, tokens)]:
+        if t == tokens - 2:
+            assert (dx[t] == 0).all()
+            continue
+        want = ref.route_grad_row(xs[t], e[t], gs[t], score, True, 2.0)
+        tol = 8e-6 * np.abs(gs[t]).max() + HALF_ULP[dtype] * np.abs(want) + 1e-7
+        assert (np.abs(dx[t].float().cpu().numpy() - want) <= tol).all(), t
+
+
 @pytest.mark.gpu
 def test_route_strides_and_no_tokens():
     big = rand(20, 131, seed=6)
@@ -209,6 +276,14 @@ def test_expert_order(tokens, k, num, popular):
     assert np.array_equal(plan.offsets.cpu().numpy(), offsets)
     assert np.array_equal(plan.order.cpu().numpy(), order)
     assert np.array_equal(plan.position.cpu().numpy(), position)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,k,num", [(1100003, 3, 1000), (9000001, 1, 2), (590001, 1, 256),
+                                          (589824, 1, 64)])
+def test_expert_order_long(tokens, k, num):
+    """Runs of several tiles, and lengths about a block's smallest run times the blocks."""
+    test_expert_order(tokens, k, num, False)
 
 
 @pytest.mark.gpu
