@@ -57,6 +57,11 @@ struct Pack {
     return Pack{*reinterpret_cast<const Raw*>(from)};
   }
   __device__ __forceinline__ void store(T* to) const { *reinterpret_cast<Raw*>(to) = raw; }
+  // for what passes once: the first to leave the caches
+  static __device__ __forceinline__ Pack load_once(const T* from) {
+    return Pack{__ldcs(reinterpret_cast<const Raw*>(from))};
+  }
+  __device__ __forceinline__ void store_once(T* to) const { __stcs(reinterpret_cast<Raw*>(to), raw); }
   __device__ __forceinline__ float value(int q) const {
     return E::to_float(reinterpret_cast<const T*>(&raw)[q]);
   }
@@ -829,9 +834,11 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(OrderParams p) {
 //
 // VEC elements a thread at a time: 16 bytes when the pointers, strides and width allow it, else one.
 // These kernels move bytes; what carries them is the number of independent loads in flight, so each
-// takes four rows at a time before the first is used.  At 8191 tokens x 6 rows of 4 KB dispatch moves
-// 235 MB in 44 us, combine 235 MB in 43 us and its backward kernel 436 MB in 79 us: 5.3 to 5.5 TB/s,
-// 81 to 84% of a plain copy's rate.
+// takes four rows at a time before the first is used.  dispatch and combine let the long side (k
+// rows a token) pass the caches, which then keep the short one.  With nothing in the caches at
+// 8191 tokens x 6 rows of 4 KB: dispatch 47 us for 235 MB (50 us without that), combine 46 us
+// for as many (55 us without that and with five blocks an SM for six), its backward kernel 82 us
+// for 436 MB (88 us with it): 5.0 to 5.3 TB/s, 77 to 81% of a plain copy's rate.
 
 constexpr int kRowThreads = 256;
 constexpr int kAhead = 4;
@@ -872,14 +879,14 @@ __global__ void __launch_bounds__(kRowThreads)
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const long long r = r0 + u * side;
-        if (r < n) v[u].store(rows + (r * nvec + c) * VEC);
+        if (r < n) v[u].store_once(rows + (r * nvec + c) * VEC);
       }
     }
   }
 }
 
 template <class E, int VEC>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 6)
     combine_kernel(const typename E::T* rows, const int* position, const float* weights,
                    typename E::T* y, int tokens, int k, int nvec) {
   using P = Pack<E, VEC>;
@@ -899,7 +906,7 @@ __global__ void __launch_bounds__(kRowThreads)
           const int a = j0 + u < k ? at[j0 + u] : -1;
           const bool in = a >= 0 && a < n;
           w[u] = in && wt ? wt[j0 + u] : 1.0f;
-          v[u] = in ? P::load(rows + (static_cast<long long>(a) * nvec + c) * VEC)
+          v[u] = in ? P::load_once(rows + (static_cast<long long>(a) * nvec + c) * VEC)
                     : zero_pack<E, VEC>();
         }
 #pragma unroll
