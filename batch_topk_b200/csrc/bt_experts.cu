@@ -838,7 +838,8 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(OrderParams p) {
 // rows a token) pass the caches, which then keep the short one.  With nothing in the caches at
 // 8191 tokens x 6 rows of 4 KB: dispatch 47 us for 235 MB (50 us without that), combine 46 us
 // for as many (55 us without that and with five blocks an SM for six), its backward kernel 82 us
-// for 436 MB (88 us with it): 5.0 to 5.3 TB/s, 77 to 81% of a plain copy's rate.
+// for 436 MB (88 us with it), launch and ramp included: 5.0 to 5.3 TB/s, 77 to 81% of a plain copy's
+// rate; without them 41, 38 and 79 us.
 
 constexpr int kRowThreads = 256;
 constexpr int kAhead = 4;
