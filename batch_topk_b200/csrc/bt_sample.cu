@@ -245,8 +245,9 @@ struct Slice {
 
   // f(index, value) for every element of the vectors of the slice whose maximum passes; four
   // vectors in flight.
+  // f(index, values) for the vectors that `pass`; places outside the row hold -inf.
   template <class P, class F>
-  __device__ __forceinline__ void each(P pass, F f) const {
+  __device__ __forceinline__ void each_vector(P pass, F f) const {
     for (int first = v0 + static_cast<int>(threadIdx.x); first < v1; first += kGroup * kThreads) {
       uint4 r[kGroup];
 #pragma unroll
@@ -261,11 +262,17 @@ struct Slice {
         if (v < v1 && pass(V::max2(now, now))) {
           float x[kPer];
           V::unpack(now, x);
-#pragma unroll
-          for (int q = 0; q < kPer; ++q) f(v * kPer + q - shift, x[q]);
+          f(v * kPer - shift, x);
         }
       }
     }
+  }
+  template <class P, class F>
+  __device__ __forceinline__ void each(P pass, F f) const {
+    each_vector(pass, [&](int i, const float (&x)[kPer]) {
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) f(i + q, x[q]);
+    });
   }
   template <class F>
   __device__ __forceinline__ void each(F f) const {
@@ -444,6 +451,12 @@ struct Sampler {
   // Bins of log-weight, in 64ths of an octave below the maximum: 256 of width 1, 256 of 2, 256 of
   // 4 and so on, taken from the exponent and mantissa of 256 + distance.  A smaller value never
   // has a smaller bin; kBins: its weight is 0 in float32 (more than 190 octaves down).
+  __device__ __forceinline__ float place(float x) const {
+    return fmaf(m - x, c * 64.0f, 256.0f);  // m is finite where this is used
+  }
+  static __device__ __forceinline__ float bin_edge(int b) {  // the place at which bin b begins
+    return __uint_as_float(__float_as_uint(256.0f) + (static_cast<uint32_t>(b) << 15));
+  }
   __device__ __forceinline__ int bin(float x) const {
     const float t = x == m ? 256.0f : fmaf(m - x, c * 64.0f, 256.0f);
     return t < 16384.0f
@@ -453,7 +466,7 @@ struct Sampler {
   // Bins [fine_of, fine_end] that hold too much are binned again, linearly in the value from their
   // upper edge; elements of the bins before them are in fine bin -1, those after them in kBins.
   int fine_of = -1, fine_end = -1;
-  float fine_top, fine_scale;
+  float fine_top = 0.0f, fine_scale = 0.0f;
   __device__ __forceinline__ void refine(int b, int end) {
     fine_of = b;
     fine_end = end;
@@ -465,7 +478,13 @@ struct Sampler {
     if (fine_of < 0 || b >= kBins) return b;
     if (b < fine_of) return -1;
     if (b > fine_end) return kBins;
+    return fine_place(x);
+  }
+  __device__ __forceinline__ int fine_place(float x) const {  // of an element of the bins binned again
     return min(max(static_cast<int>((fine_top - x) * fine_scale), 0), kBins - 1);
+  }
+  static __device__ __forceinline__ int coarse_place(float t) {  // beyond kBins for what has none
+    return static_cast<int>((__float_as_uint(t) - __float_as_uint(256.0f)) >> 15);
   }
 
   // Distance, in 64ths of an octave, at which bin b begins.
@@ -1053,6 +1072,33 @@ struct Sampler {
     return best;
   }
 
+  // weigh_one() of the elements of the bins up to `last` (the fine ones if FINE), a vector at a time and
+  // without branches up to the counting.
+  template <bool FINE>
+  __device__ __forceinline__ void weigh_vectors(float low, int last, float units) {
+    const float begin = bin_edge(FINE ? fine_of : 0), end = bin_edge(last + 1);
+    s.each_vector([&](float x) { return x >= low; }, [&](int, const float (&x)[kPer]) {
+      float t[kPer];
+      int b[kPer];
+      uint32_t w[kPer];
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        t[q] = place(x[q]);
+        b[q] = FINE ? fine_place(x[q]) : coarse_place(t[q]);
+        // what a bin's number leaves of the place is the distance from its start
+        const float from = FINE ? begin : __uint_as_float(__float_as_uint(t[q]) & 0xFFFF8000u);
+        w[q] = static_cast<uint32_t>(exp2_approx((t[q] - from) * (-1.0f / 64.0f)) * units + 0.5f);
+      }
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        if (t[q] >= begin && t[q] < end) {
+          atomicAdd(&sh.bins[b[q]], 1u);
+          atomicAdd(&sh.weights[b[q]], w[q]);
+        }
+      }
+    });
+  }
+
   // Pass 2 of an overflowing row: counts and weights by bin of the elements of the bins up to
   // `last`, joined in every block; then sh.bin is the bin that holds the cut.
   // `above` elements of weight `heavier` lie before the bins that are looked through.
@@ -1061,10 +1107,8 @@ struct Sampler {
     clear_bins();
     __syncthreads();
     const float low = bin_floor(last);
-    s.each([&](float x) { return x >= low; },
-           [&](int, float x) {
-             if (x >= low && bin(x) <= last) weigh_one(x, units);
-           });
+    if (fine_of < 0) weigh_vectors<false>(low, last, units);
+    else weigh_vectors<true>(low, last, units);
     team.sync();
     if (team.blocks > 1) {  // block b joins its share of the bins from all, and gives it to all
       const int share = (kBins + team.blocks - 1) / team.blocks;
@@ -1091,6 +1135,57 @@ struct Sampler {
     }
   }
 
+  // split()'s pass over the row.
+  template <bool FINE>
+  __device__ __forceinline__ void split_vectors(float low, int at, int end, float& za, float& zi,
+                                                uint32_t& n, Race& run) {
+    // A vector at a time: its noise is loaded at once, and raced where an element may lead.
+    const float fine_from = bin_edge(FINE ? fine_of : 0), fine_to = bin_edge(fine_end + 1);
+    s.each_vector([&](float x) { return x >= low; }, [&](int i, const float (&x)[kPer]) {
+      float w[kPer], d[kPer];
+      uint32_t over = 0, in = 0;  // the elements above the bins, and in them
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        const float t = place(x[q]);
+        int b = FINE ? fine_place(x[q]) : coarse_place(t);
+        if (FINE) b = t < fine_from ? -1 : (t < fine_to ? b : kBins);
+        over |= b < at ? 1u << q : 0u;
+        in |= b >= at && b <= end ? 1u << q : 0u;
+      }
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        w[q] = (over >> q) & 1u ? weight_near(x[q]) : 0.0f;
+        d[q] = (over >> q) & 1u ? __ldg(noise + i + q) : 1.0f;
+      }
+      n += __popc(over);
+      bool leads = false;
+      const float lead = 0.9999f * run.lead;
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        za += w[q];
+        leads |= ((over >> q) & 1u) && !(w[q] < lead * d[q]);
+      }
+      if (leads) {
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+          if (((over >> q) & 1u) && (!(min_p > 0.0f) || !(weight(x[q]) < min_p))) {
+            race(run, x[q], i + q, w[q]);
+          }
+        }
+      }
+      if (in) {
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+          if ((in >> q) & 1u) {
+            zi += weight_near(x[q]);
+            const uint32_t to = atomicAdd(&sh.count, 1u);
+            if (to < kCap) put(to, i + q, x[q]);
+          }
+        }
+      }
+    });
+  }
+
   // Pass 3: the elements of the bins [at, end] into the list; those above them are all kept, so
   // they are counted, summed and raced.  `inside`: the weight in the bins.
   __device__ __forceinline__ uint32_t split_in(int at, int end, Sum* above, double* inside,
@@ -1100,21 +1195,8 @@ struct Sampler {
     uint32_t n = 0;
     Race run;
     const float low = bin_floor(fine_of < 0 ? end : fine_end);
-    s.each([&](float x) { return x >= low; }, [&](int i, float x) {
-      if (!(x >= low)) return;
-      const int b = fine_bin(x);
-      if (b > end) return;
-      const float w = weight_near(x);
-      if (b >= at) {
-        zi += w;
-        const uint32_t to = atomicAdd(&sh.count, 1u);
-        if (to < kCap) put(to, i, x);
-      } else {
-        za += w;
-        ++n;
-        if (!(min_p > 0.0f) || !(weight(x) < min_p)) race(run, x, i, w);
-      }
-    });
+    if (fine_of < 0) split_vectors<false>(low, at, end, za, zi, n, run);
+    else split_vectors<true>(low, at, end, za, zi, n, run);
     float unused;
     const uint32_t listed = close_list(0.0f, &unused);
     *above = team.sum(za, n);
@@ -1433,60 +1515,80 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(const __
   if (team.blocks > 1) team.cluster.sync();  // no block leaves while another may read its parts
 }
 
-std::mutex g_mu;  // over what is set once per device
+std::mutex g_mu;  // over what is looked up once per device
 
 template <class E>
-int launch(Params p, int blocks, cudaStream_t stream) {
+cudaLaunchConfig_t config(int rows, int blocks, int smem, cudaLaunchAttribute* attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = blocks;
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+constexpr int kSlotBytes = kThreads * static_cast<int>(sizeof(float));
+
+// Once per device: shared memory beyond the default, and how many clusters of each size it runs at a
+// time.
+template <class E>
+static int ready(const int** fits) {  // static, so that `known` is this library's own
+  static int known[64][kMaxCluster + 1] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(g_mu);
+  int* fit = known[dev];
+  if (!fit[0]) {
+    constexpr int kSmem = static_cast<int>(sizeof(Shared)) + kMaxSlots * kSlotBytes;
+    e = cudaFuncSetAttribute(sample_kernel<E>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    for (int blocks = 1; blocks <= kMaxCluster; ++blocks) {
+      cudaLaunchAttribute attr;
+      const cudaLaunchConfig_t cfg = config<E>(1, blocks, kSmem, &attr);
+      e = cudaOccupancyMaxActiveClusters(&fit[blocks], sample_kernel<E>, &cfg);
+      if (e != cudaSuccess) return e;
+    }
+    fit[0] = 1;
+  }
+  *fits = fit;
+  return 0;
+}
+
+// Blocks a row: as many as let all rows run at once, but no more than leave each thread a vector.
+// A block too many costs a second wave: 64 rows of 128256, top-p, take 18 us with 6 blocks a row and
+// 26 us with 8, 120 rows 22 us with 3 and 30 us with 4.
+int blocks_for(const int* fits, int rows, int vocab, int per) {
+  int blocks = kMaxCluster;
+  while (blocks > 1 && (rows > fits[blocks] || (blocks - 1) * kThreads * per >= vocab)) --blocks;
+  return blocks;
+}
+
+template <class E>
+int launch(Params p, cudaStream_t stream) {
   constexpr int kPer = Vec<E>::kPer;
+  const int* fits;
+  if (const int rc = ready<E>(&fits)) return rc;
+  const int blocks = blocks_for(fits, p.rows, p.vocab, kPer);
   const long long vecs = (static_cast<long long>(p.vocab) + 2 * kPer - 2) / kPer;
   const long long per = (vecs + blocks - 1) / blocks;
   const long long groups = (per + kGroup * kThreads - 1) / (kGroup * kThreads);
   p.groups_per_slot = static_cast<int>((groups + kMaxSlots - 1) / kMaxSlots);
   p.slots = static_cast<int>((groups + p.groups_per_slot - 1) / p.groups_per_slot);
-  const int slot_bytes = kThreads * static_cast<int>(sizeof(float));
-  const int smem = static_cast<int>(sizeof(Shared)) + p.slots * slot_bytes;
-  static bool known[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  {
-    std::lock_guard<std::mutex> lock(g_mu);
-    if (!known[dev]) {
-      e = cudaFuncSetAttribute(sample_kernel<E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(sizeof(Shared)) + kMaxSlots * slot_bytes);
-      if (e != cudaSuccess) return e;
-      known[dev] = true;
-    }
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * blocks);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  cudaLaunchConfig_t cfg =
+      config<E>(p.rows, blocks, static_cast<int>(sizeof(Shared)) + p.slots * kSlotBytes, &attr);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = blocks;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, sample_kernel<E>, p);
 }
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
-
-// Blocks a row: as many as give each of 148 SMs two blocks, but no more than leave each thread a
-// vector.  More blocks finish a row sooner but pay for their exchanges: 200 rows of 151936 without
-// filters take 56, 41, 46 and 67 us with 1, 2, 4 and 8 blocks a row.
-int blocks_for(int rows, int vocab, int per) {
-  int blocks = 1;
-  while (blocks < kMaxCluster && static_cast<long long>(rows) * blocks < 2 * 148 &&
-         static_cast<long long>(vocab) > static_cast<long long>(blocks) * kThreads * per) {
-    blocks *= 2;
-  }
-  return blocks;
-}
 
 }  // namespace bts
 
@@ -1510,11 +1612,10 @@ extern "C" int bt_sample(const void* d_logits, int elem, int rows, int vocab,
   Params p{d_logits, logits_stride, d_noise, noise_stride, temperature, top_p, min_p, top_k,
            d_temperature, d_top_p, d_min_p, d_top_k, d_tokens, d_logprobs, rows, vocab, 0, 0};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int blocks = blocks_for(rows, vocab, static_cast<int>(16 / es));
   switch (elem) {
-    case BT_DTYPE_F16: return launch<Elem<__half>>(p, blocks, s);
-    case BT_DTYPE_BF16: return launch<Elem<__nv_bfloat16>>(p, blocks, s);
-    case BT_DTYPE_F32: return launch<Elem<float>>(p, blocks, s);
+    case BT_DTYPE_F16: return launch<Elem<__half>>(p, s);
+    case BT_DTYPE_BF16: return launch<Elem<__nv_bfloat16>>(p, s);
+    case BT_DTYPE_F32: return launch<Elem<float>>(p, s);
     default: return cudaErrorInvalidValue;
   }
 }
