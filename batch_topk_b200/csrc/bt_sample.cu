@@ -316,6 +316,7 @@ struct Shared {
   int bin, bin_end;        // found by find_bin: the bins that may hold the target,
   uint32_t above, inside;  // the elements before them, and in them
   float heavier;           // the weight before them
+  float others;            // see others_in(); negative where it was not needed
 };
 
 // Every block reads all blocks' parts in rank order, so all of them hold the same bits and take
@@ -748,6 +749,42 @@ struct Sampler {
     }
     m = w.x;
     z = w.y * exp2_approx(-fmaf(m, c, -__fmul_rn(m, c)));
+  }
+
+  // Where one element has most of the weight its log-probability -log(z) is near 0, and the rounding
+  // of sums above 1 is all of its error.  sh.others becomes the sum without the maximum: that of the
+  // other threads, and the one's that holds the maximum from its vectors, read again by the block.
+  __device__ __forceinline__ void others_in(float mt, float zt, bool whole) {
+    if (threadIdx.x == 0) sh.hot_count = ~0u;
+    __syncthreads();
+    if (mt == m) sh.hot_count = threadIdx.x;  // one thread of the row: z is below 2
+    __syncthreads();
+    const uint32_t owner = sh.hot_count;
+    const float mc = __fmul_rn(m, c);
+    float sum = 0.0f;
+    if (mt > kNegInf && mt < m) {
+      sum = zt * exp2_approx(__fmul_rn(mt, c) - mc) * exp2_approx(-fmaf(m, c, -mc));
+    }
+    auto add = [&](int v) {
+      const uint4 r = V::clean(s.fix(v, s.raw(v)));
+      float x[kPer];
+      V::unpack(r, x);
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) sum += x[q] == m ? 0.0f : weight_near(x[q]);
+    };
+    if (owner != ~0u) {
+      const int first = (whole ? s.v0 : s.i0) + static_cast<int>(owner), end = whole ? s.v1 : s.i1;
+      for (long long v = first + static_cast<long long>(threadIdx.x) * kThreads; v < end;
+           v += kThreads * kThreads) {
+        add(static_cast<int>(v));
+      }
+      if (!whole && threadIdx.x == 0 && owner < 2) {  // the row's first and last vectors
+        const int v = owner == 0 ? 0 : s.vecs - 1;
+        if (v >= s.v0 && v < s.v1 && (owner == 0 || v > 0)) add(v);
+      }
+    }
+    const Sum all = team.sum(sum, 0);
+    if (threadIdx.x == 0) sh.others = static_cast<float>(all.mass);
   }
 
   __device__ __forceinline__ void clear_bins() {
@@ -1333,12 +1370,16 @@ struct Sampler {
     return best;
   }
 
+  __device__ __noinline__ void others(float mt, float zt, bool whole) const {
+    Sampler me(*this);
+    me.others_in(mt, zt, whole);
+  }
   __device__ __forceinline__ void write(u64 best, float total, long long r) const {
     const int token = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(best));
     const float x = fmaxf(
         E::to_float(static_cast<const typename E::T*>(p.logits)[r * p.stride + token]), kNegInf);
     p.tokens[r] = token;
-    p.logprobs[r] = scaled(x) - logf(total);
+    p.logprobs[r] = x == m && sh.others >= 0.0f ? -log1pf(sh.others) : scaled(x) - logf(total);
   }
 };
 
@@ -1381,7 +1422,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(const __
 
   const bool open_race = !one && !by_k && !by_p && !by_m;
   sh.runs[threadIdx.x] = 0;
-  if (threadIdx.x == 0) sh.count = sh.total = 0;  // an open list, seen by all after join()
+  if (threadIdx.x == 0) {
+    sh.count = sh.total = 0;  // an open list, seen by all after join()
+    sh.others = -1.0f;
+  }
   float mt, zt, wx = 0.0f;
   int wi = -1;
   if (open_race) {
@@ -1402,6 +1446,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(const __
       p.logprobs[r] = kNegInf;
     }
     return;
+  }
+  if (k.z > 0.5f && k.z < 1.0625f && k.m < INFINITY) {  // else z is near enough: 3e-6 of log(z)
+    Sampler<E> slow = k;
+    slow.others(mt, zt, open_race);
+    k.team.parity ^= 1;
   }
   u64 best = 0;
   float total = k.z;

@@ -317,3 +317,29 @@ def test_abi_argument_errors():
     assert call(dt=FAKE + 2) == INVALID
     assert call(dk=FAKE + 1) == INVALID
     assert call(lp=FAKE + 2) == INVALID
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [37, 1000, 32003, 128256])
+@pytest.mark.parametrize("settings", [dict(), dict(temperature=0.0), dict(temperature=0.7, top_p=0.9),
+                                      dict(top_k=40), dict(top_k=20, top_p=0.95, min_p=0.1)])
+def test_confident_rows(dtype, vocab, settings):
+    """One token with nearly all weight: its log-probability is the others' weight.  An exponent of up
+    to 32 octaves passes through about four roundings of 2^-20, so 1e-5 of the value."""
+    n = 9
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn((n, vocab + 3), generator=g, device="cuda").to(DTYPES[dtype])[:, 1:vocab + 1]
+    at = torch.tensor([0, 1, 5, vocab // 2, vocab // 3, vocab - 1, vocab - 2, 20, 36], device="cuda")
+    lift = np.log(vocab) + torch.tensor([2.5, 4, 6, 8, 2.5, 3, 4, 10, 1.9], device="cuda")
+    x[torch.arange(n), at] = lift.to(x.dtype)
+    noise = torch.ones((n, vocab), device="cuda")  # the heaviest token wins
+    tokens, logprobs = api.sample(x, noise, **settings)
+    assert torch.equal(tokens.long(), at)
+    t = settings.get("temperature", 1.0) or 1.0
+    rows = x.double().cpu().numpy()
+    for r in range(n):
+        e = np.exp((rows[r] - rows[r, at[r]]) / np.float64(np.float32(t)))
+        e[at[r].item()] = 0.0
+        want = -np.log1p(e.sum())
+        assert abs(logprobs[r].item() - want) <= 1e-5 * abs(want), (r, logprobs[r].item(), want)
