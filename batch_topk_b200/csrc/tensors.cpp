@@ -10,10 +10,10 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/Allocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
-#include <map>
 #include <string>
 #include <utility>
 
@@ -325,18 +325,6 @@ PyObject* route(PyObject* const* a) {
 
 // ---- the experts' rows -------------------------------------------------------------------------
 
-// Scratch of a device's stream, grown as needed: calls on one stream run in order, so they may share
-// it; calls on different streams never do.  Never freed: the driver may be gone when the process
-// ends.
-at::Tensor& workspace(const at::Tensor& like, void* stream, size_t bytes) {
-  static auto* kept = new std::map<std::pair<int, void*>, at::Tensor>();
-  at::Tensor& w = (*kept)[{like.get_device(), stream}];
-  if (!w.defined() || static_cast<size_t>(w.numel()) < bytes) {
-    w = empty({static_cast<int64_t>(bytes < (1u << 18) ? (1u << 18) : bytes)}, like, at::kByte);
-  }
-  return w;
-}
-
 // expert_order(experts, num_experts)
 PyObject* expert_order(PyObject* const* a) {
   const at::Tensor& given = tensor(a[0], "experts");
@@ -360,10 +348,12 @@ PyObject* expert_order(PyObject* const* a) {
   } else {
     const at::Tensor experts = given.contiguous();
     const size_t bytes = bt_expert_order_workspace_size(static_cast<int>(n), static_cast<int>(num));
-    at::Tensor& ws = workspace(given, place.stream, bytes);
+    // The call's own: it goes back to the allocator in the stream's order, and what a CUDA graph
+    // captured belongs to that graph.
+    const c10::DataPtr scratch = c10::GetAllocator(at::kCUDA)->allocate(bytes);
     check(bt_expert_order(experts.data_ptr<int>(), static_cast<int>(n), static_cast<int>(num),
                           offsets.data_ptr<int>(), order.data_ptr<int>(), position.data_ptr<int>(),
-                          ws.data_ptr(), static_cast<size_t>(ws.numel()), place.stream),
+                          scratch.get(), bytes, place.stream),
           "expert_order");
   }
   PyObject* t = PyTuple_New(3);

@@ -533,3 +533,58 @@ def test_abi_argument_errors():
     for kw in (dict(g=0), dict(pos=0), dict(dr=0, dw=0), dict(r=0), dict(live=0), dict(gs=-1),
                dict(t=0), dict(width=0), dict(dr=FAKE + 1), dict(dw=FAKE + 2)):
         assert cback(**kw) == INVALID, kw
+
+
+@pytest.mark.gpu
+def test_expert_order_keeps_no_memory():
+    """A call's scratch is its own and goes back to the allocator with it."""
+    e = make_experts(9001, 8, 512, 1)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        before = torch.cuda.memory_allocated()
+        plan = api.expert_order(e, 512)
+        del plan
+        assert torch.cuda.memory_allocated() == before
+
+
+@pytest.mark.gpu
+def test_expert_order_in_graphs():
+    """Graphs captured on one stream, replayed beside each other, beside calls on that stream and
+    after larger ones there; nothing is written to memory that others hold by then."""
+    stream, other = torch.cuda.Stream(), torch.cuda.Stream()
+    inputs = [make_experts(16001, 8, 256, s) for s in (1, 2)]
+    want = [ref.order(e.cpu().numpy(), 256) for e in inputs]
+    large = make_experts(150001, 4, 1024, 3)
+    large_want = ref.order(large.cpu().numpy(), 1024)
+    graphs, plans = [], []
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for e in inputs:
+            api.expert_order(e, 256)
+    for e in inputs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            plans.append(api.expert_order(e, 256))
+        graphs.append(graph)
+
+    def check(plan, expected):
+        for got, exp in zip(plan, expected):
+            assert np.array_equal(got.cpu().numpy(), exp)
+
+    with torch.cuda.stream(stream):
+        check(api.expert_order(large, 1024), large_want)
+        held = [torch.zeros(1 << 18, dtype=torch.uint8, device="cuda") for _ in range(32)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        with torch.cuda.stream(stream):
+            graphs[0].replay()
+            eager = api.expert_order(large, 1024)
+        with torch.cuda.stream(other):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        check(eager, large_want)
+        for plan, expected in zip(plans, want):
+            check(plan, expected)
+            for t in plan:
+                t.fill_(-7)
+    torch.cuda.synchronize()
+    assert not any(t.any().item() for t in held)
