@@ -988,7 +988,8 @@ __global__ void __launch_bounds__(kRowThreads, 5)
 #pragma unroll
         for (int u = 0; u < kBackRows; ++u) {
           dot[u] = lanes_sum(dot[u]);
-          if (lane == 0) part[warp][u] = dot[u];
+          // without a row the products were with 0: NaN where the gradient is not finite
+          if (lane == 0) part[warp][u] = at[u] >= 0 ? dot[u] : 0.0f;
         }
         __syncthreads();
         if (threadIdx.x < kBackRows && j0 + threadIdx.x < static_cast<unsigned>(k)) {

@@ -588,3 +588,22 @@ def test_expert_order_in_graphs():
                 t.fill_(-7)
     torch.cuda.synchronize()
     assert not any(t.any().item() for t in held)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [64, 4099])
+def test_combine_gradient_of_absent_assignments(dtype, width):
+    """Gradients of infinities and NaN: a weight without a row still has gradient 0."""
+    experts = torch.tensor([[0, -1, 2], [-1, -1, -1], [1, 2, -1]], dtype=torch.int32, device="cuda")
+    plan = api.expert_order(experts, 3)
+    rows = rand(9, width, seed=1, dtype=dtype).requires_grad_()
+    weights = rand(3, 3, seed=2).requires_grad_()
+    g = rand(3, width, seed=3, dtype=dtype)
+    g[0, 5] = float("inf")
+    g[1, 7] = float("nan")
+    g[2, 0] = -float("inf")
+    d_rows, d_weights = torch.autograd.grad(api.combine(rows, plan, weights), (rows, weights), g)
+    absent = experts < 0
+    assert (d_weights[absent] == 0).all() and not torch.isfinite(d_weights[~absent]).any()
+    assert (d_rows[4:] == 0).all()  # five of nine places are empty
