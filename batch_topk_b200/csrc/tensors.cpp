@@ -11,6 +11,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/Allocator.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -55,11 +56,21 @@ void check(int code, const char* what) {
   if (code != 0) throw Failed(code, what);
 }
 
+// A dual tensor's tangent would be lost.
+void no_tangent(const at::Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(0).defined() ||
+                  !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
+              "route, dispatch and combine have no forward-mode derivatives");
+}
 void first_order(const at::Tensor& grad) {
+  no_tangent(grad);
   TORCH_CHECK(!(at::GradMode::is_enabled() && grad.requires_grad()),
               "route, dispatch and combine have first-order gradients only");
 }
-bool wants_grad(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+bool wants_grad(const at::Tensor& t) {
+  no_tangent(t);
+  return t.requires_grad() && at::GradMode::is_enabled();
+}
 
 PyObject* raise(const Refused& r) {
   PyErr_SetString(PyExc_ValueError, r.what());
@@ -499,7 +510,8 @@ PyObject* combine(PyObject* const* a) {
       weights.device() != rows.device()) {
     refuse("weights must be a float32 tensor of plan.position's shape on the rows' device");
   }
-  if (wants_grad(rows) || wants_grad(weights)) {
+  const bool for_rows = wants_grad(rows), for_weights = wants_grad(weights);
+  if (for_rows || for_weights) {
     return THPVariable_Wrap(CombineNode::apply(rows, weights, plan));
   }
   return THPVariable_Wrap(combine_forward(rows, plan.position, weights.contiguous()));

@@ -607,3 +607,25 @@ def test_combine_gradient_of_absent_assignments(dtype, width):
     absent = experts < 0
     assert (d_weights[absent] == 0).all() and not torch.isfinite(d_weights[~absent]).any()
     assert (d_rows[4:] == 0).all()  # five of nine places are empty
+
+
+@pytest.mark.gpu
+def test_forward_mode_derivatives_are_refused():
+    """A tangent that the operators cannot carry on is not dropped."""
+    import torch.autograd.forward_ad as forward_ad
+
+    x, weights = rand(4, 16, seed=1), rand(4, 2, seed=2)
+    plan = api.expert_order(make_experts(4, 2, 8, 1), 8)
+    rows = api.dispatch(x, plan)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: api.route(dual(x), 2), lambda: api.dispatch(dual(x), plan),
+                     lambda: api.combine(dual(rows), plan, weights),
+                     lambda: api.combine(rows, plan, dual(weights))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        weights, _ = api.route(x.requires_grad_(), 2)  # a level alone changes nothing
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(weights, x, dual(torch.ones((4, 2), device="cuda")))
