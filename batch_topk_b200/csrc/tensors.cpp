@@ -72,6 +72,22 @@ bool wants_grad(const at::Tensor& t) {
   return t.requires_grad() && at::GradMode::is_enabled();
 }
 
+// A gradient under create_graph, which depends on `source` beside the upstream gradient: the same
+// values with a node that refuses to be differentiated, so that no term is dropped on the way to
+// source.
+struct OnceNode : torch::autograd::Function<OnceNode> {
+  static at::Tensor forward(AutogradContext*, const at::Tensor& gradient, const at::Tensor&) {
+    return gradient.alias();
+  }
+  static variable_list backward(AutogradContext*, const variable_list&) {
+    TORCH_CHECK(false, "route, dispatch and combine have first-order gradients only");
+  }
+};
+at::Tensor once(const at::Tensor& gradient, const at::Tensor& source) {
+  const bool graph = gradient.defined() && at::GradMode::is_enabled() && source.requires_grad();
+  return graph ? OnceNode::apply(gradient, source) : gradient;
+}
+
 PyObject* raise(const Refused& r) {
   PyErr_SetString(PyExc_ValueError, r.what());
   return nullptr;
@@ -290,7 +306,7 @@ struct RouteNode : torch::autograd::Function<RouteNode> {
                               place.stream),
             "route backward");
     }
-    return {out, at::Tensor()};
+    return {once(out, saved[0]), at::Tensor()};
   }
 };
 
@@ -479,7 +495,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
     } else if (d_weights.defined()) {
       d_weights.zero_();
     }
-    return {d_rows, d_weights, at::Tensor()};
+    return {once(d_rows, saved[1]), once(d_weights, saved[0]), at::Tensor()};
   }
 };
 

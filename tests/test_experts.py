@@ -629,3 +629,34 @@ def test_forward_mode_derivatives_are_refused():
         weights, _ = api.route(x.requires_grad_(), 2)  # a level alone changes nothing
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(weights, x, dual(torch.ones((4, 2), device="cuda")))
+
+
+@pytest.mark.gpu
+def test_second_order_terms_are_not_dropped():
+    """Gradients taken with create_graph and a constant upstream gradient are those of the first
+    order; differentiating them again is refused, also where another path gives a gradient."""
+    x, one = rand(4, 16, seed=1).requires_grad_(), torch.ones((4, 2), device="cuda")
+    want, = torch.autograd.grad(api.route(x, 2)[0], x, one)
+    dx, = torch.autograd.grad(api.route(x, 2)[0], x, one, create_graph=True)
+    assert torch.equal(dx, want)
+    for differentiate in (lambda v: v.backward(), lambda v: torch.autograd.grad(v, x)):
+        dx, = torch.autograd.grad(api.route(x, 2)[0], x, one, create_graph=True)
+        with pytest.raises(RuntimeError, match="first-order"):
+            differentiate(dx.square().sum() + x.square().sum())
+
+    plan = api.expert_order(make_experts(4, 2, 8, 1), 8)
+    rows, weights = rand(8, 16, seed=2).requires_grad_(), rand(4, 2, seed=3).requires_grad_()
+    g = rand(4, 16, seed=4)
+    want = torch.autograd.grad(api.combine(rows, plan, weights), (rows, weights), g)
+    got = torch.autograd.grad(api.combine(rows, plan, weights), (rows, weights), g,
+                              create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for d, source in ((got[0], weights), (got[1], rows)):
+        with pytest.raises(RuntimeError, match="first-order"):
+            torch.autograd.grad(d.sum() + source.sum(), source, retain_graph=True)
+    # the gradient of rows under constant weights, and dispatch's, depend on nothing more
+    d_rows, = torch.autograd.grad(api.combine(rows, plan, weights.detach()), rows, g,
+                                  create_graph=True)
+    assert torch.equal(d_rows, want[0]) and not d_rows.requires_grad
+    d_x, = torch.autograd.grad(api.dispatch(x, plan), x, rand(8, 16, seed=5), create_graph=True)
+    assert not d_x.requires_grad
