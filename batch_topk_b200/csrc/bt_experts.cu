@@ -1026,7 +1026,7 @@ int launch_route(const RouteParams& p, cudaStream_t s) {
   constexpr int kTokens = kRouteWarps * 32 / L;
   const bool wide = p.num == L * NPL && p.stride % kPer == 0 &&
                     aligned(p.logits, sizeof(T) * kPer) && aligned(p.bias, 16);
-  const int grid = (p.tokens + kTokens - 1) / kTokens;
+  const unsigned grid = (static_cast<unsigned>(p.tokens) + kTokens - 1) / kTokens;
   if (wide) route_kernel<E, NPL, true, L><<<grid, 32 * kRouteWarps, 0, s>>>(p);
   else route_kernel<E, NPL, false, L><<<grid, 32 * kRouteWarps, 0, s>>>(p);
   return cudaGetLastError();
@@ -1038,7 +1038,7 @@ int launch_route(const RouteBackParams& p, cudaStream_t s) {
   constexpr int kTokens = kRouteWarps * 32 / L;
   const bool wide = p.num == L * NPL && p.stride % kPer == 0 &&
                     aligned(p.logits, sizeof(T) * kPer) && aligned(p.d_logits, sizeof(T) * kPer);
-  const int grid = (p.tokens + kTokens - 1) / kTokens;
+  const unsigned grid = (static_cast<unsigned>(p.tokens) + kTokens - 1) / kTokens;
   if (wide) route_backward_kernel<E, NPL, true, L><<<grid, 32 * kRouteWarps, 0, s>>>(p);
   else route_backward_kernel<E, NPL, false, L><<<grid, 32 * kRouteWarps, 0, s>>>(p);
   return cudaGetLastError();

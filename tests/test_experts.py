@@ -660,3 +660,15 @@ def test_second_order_terms_are_not_dropped():
     assert torch.equal(d_rows, want[0]) and not d_rows.requires_grad
     d_x, = torch.autograd.grad(api.dispatch(x, plan), x, rand(8, 16, seed=5), create_graph=True)
     assert not d_x.requires_grad
+
+
+@pytest.mark.gpu
+def test_route_of_the_largest_number_of_tokens():
+    """2^31 - 1 tokens (one row of logits for all): the number of blocks passes through no overflow."""
+    n = 2**31 - 1
+    x = torch.zeros((1, 2), dtype=torch.float16, device="cuda").expand(n, 2).requires_grad_()
+    weights, experts = api.route(x, 1, score="sigmoid", renormalize=False)
+    dx, = torch.autograd.grad(weights, x, torch.ones((1, 1), device="cuda").expand(n, 1))
+    for t in (slice(0, 100), slice(n // 2, n // 2 + 100), slice(n - 100, n)):
+        assert (experts[t] == 0).all() and (weights[t] == 0.5).all()
+        assert (dx[t, 0] == 0.25).all() and (dx[t, 1] == 0).all()
