@@ -165,6 +165,11 @@ double number(PyObject* o) {
   if (v == -1.0 && PyErr_Occurred()) throw python_error();
   return v;
 }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw python_error();
+  return v != 0;
+}
 
 // ---- sampling --------------------------------------------------------------------------------
 
@@ -248,6 +253,7 @@ PyObject* sample(PyObject* const* a) {
 
 int score_of(PyObject* o) {
   const char* name = PyUnicode_Check(o) ? PyUnicode_AsUTF8(o) : "";
+  if (!name) throw python_error();  // a UnicodeEncodeError, which is a ValueError
   if (std::string("softmax") == name) return BT_SCORE_SOFTMAX;
   if (std::string("sigmoid") == name) return BT_SCORE_SIGMOID;
   refuse("score must be \"softmax\" or \"sigmoid\", got \"", name, "\"");
@@ -339,7 +345,7 @@ PyObject* route(PyObject* const* a) {
     bias = bias.contiguous();
   }
   const RouteArgs args{elem, static_cast<int>(k), score, static_cast<int>(groups),
-                       static_cast<int>(topk_groups), PyObject_IsTrue(a[6]),
+                       static_cast<int>(topk_groups), truth(a[6]),
                        static_cast<float>(number(a[7])), bias};
   small(tokens, "the number of tokens");
   if (wants_grad(given)) {

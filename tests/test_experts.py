@@ -672,3 +672,17 @@ def test_route_of_the_largest_number_of_tokens():
     for t in (slice(0, 100), slice(n // 2, n // 2 + 100), slice(n - 100, n)):
         assert (experts[t] == 0).all() and (weights[t] == 0.5).all()
         assert (dx[t, 0] == 0.25).all() and (dx[t, 1] == 0).all()
+
+
+@pytest.mark.gpu
+def test_arguments_that_cannot_be_read():
+    """An error raised while an argument is read is the call's error."""
+    class Unclear:
+        def __bool__(self):
+            raise ZeroDivisionError
+
+    x = rand(4, 16, seed=1)
+    with pytest.raises(ZeroDivisionError):
+        api.route(x, 2, renormalize=Unclear())
+    with pytest.raises(ValueError):
+        api.route(x, 2, score="\ud800")
