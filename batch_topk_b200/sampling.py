@@ -31,8 +31,8 @@ def sample(logits: torch.Tensor, noise: torch.Tensor, *, temperature=1.0, top_k=
         return tensors().sample(logits, noise, temperature, top_k, top_p, min_p, out)
     if stream.device != logits.device:
         raise ValueError(f"stream is on {stream.device}, the input on {logits.device}")
-    for x in (logits, noise, temperature, top_k, top_p, min_p):
+    for x in (logits, noise, temperature, top_k, top_p, min_p, *(out if isinstance(out, tuple) else ())):
         if isinstance(x, torch.Tensor) and x.is_cuda:
-            x.record_stream(stream)  # read there: keep its memory until the stream has run
+            x.record_stream(stream)  # used there: keep its memory until the stream has run
     with torch.cuda.stream(stream):
         return tensors().sample(logits, noise, temperature, top_k, top_p, min_p, out)

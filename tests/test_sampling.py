@@ -343,3 +343,19 @@ def test_confident_rows(dtype, vocab, settings):
         e[at[r].item()] = 0.0
         want = -np.log1p(e.sum())
         assert abs(logprobs[r].item() - want) <= 1e-5 * abs(want), (r, logprobs[r].item(), want)
+
+
+@pytest.mark.gpu
+def test_outputs_given_for_another_stream_are_kept_for_it(monkeypatch):
+    """What a call on another stream reads or writes is not handed out again before it has run."""
+    kept = []
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: kept.append((t.data_ptr(), s)))
+    x, q = inputs(4, 100, "fp32", 3)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    out = (torch.empty(4, dtype=torch.int32, device="cuda"), torch.empty(4, device="cuda"))
+    p = torch.full((4,), 0.9, device="cuda")
+    api.sample(x, q, top_p=p, stream=side, out=out)
+    side.synchronize()
+    for t in (x, q, p, *out):
+        assert (t.data_ptr(), side) in kept
