@@ -668,19 +668,20 @@ struct Sampler {
     }
   }
 
-  // Pass 1 without filters: the race runs along.  Within a thread quotients are compared in the
-  // approximate weights (relative to the thread's maximum), so two elements of one thread whose
-  // quotients agree to about 2^-20 may change places; the threads' winners are compared exactly.
+  // Pass 1 without filters: the race runs along.  A thread keeps the lead among its elements in
+  // approximate weights, relative to its maximum, and whether another element came within 1e-4 of
+  // it (the approximation is within 1e-5): then settle() compares exactly.
   // Bound by memory: 6 bytes an element (16-bit logits) at 4.4 TB/s, 200 rows of 151936 in 41 us.
   struct Racer {
     float top, sum, x;
-    int at;
+    int at;  // 2 * index, + 1 where another was as near; negative without any
   };
   static __device__ __noinline__ Racer scan_race(const S s, const float* noise, float c) {
     const bool wide = s.shift == 0 && reinterpret_cast<uintptr_t>(noise) % (4 * kPer) == 0;
-    float mt = kNegInf, wx = kNegInf;
+    float mt = kNegInf, wx = kNegInf, wq = 1.0f;  // the maximum; the lead's logit and noise
     int wi = -1;
-    float ref = kNegInf, z0 = 0.0f, z1 = 0.0f, lead = 0.0f;
+    bool close = false;
+    float ref = kNegInf, z0 = 0.0f, z1 = 0.0f, bar = 0.0f;  // bar: 0.9999 of the lead's quotient
     int v = s.v0 + static_cast<int>(threadIdx.x);
     uint4 r = s.raw(v);
     float next[kPer];
@@ -700,7 +701,8 @@ struct Sampler {
         const float f = exp2_approx(old - ref);
         z0 *= f;
         z1 *= f;
-        lead *= f;
+        // anew: a product for every new maximum would add up its errors
+        bar = 0.9999f * __fdividef(exp2_approx(fmaf(wx, c, -ref)), wq);
       }
       if (most > kNegInf) {
         float x[kPer];
@@ -709,15 +711,35 @@ struct Sampler {
         for (int h = 0; h < kPer; ++h) {
           const float w = exp2_approx(fmaf(x[h], c, -ref));
           if (h & 1) z1 += w; else z0 += w;
-          if (w > lead * q[h] && q[h] >= 0.0f) {
-            lead = __fdividef(w, q[h]);
-            wx = x[h];
-            wi = v * kPer + h - s.shift;
+          if (w > bar * q[h] && q[h] >= 0.0f) {
+            const float high = 0.9999f * __fdividef(w, q[h]);
+            close = !(high > 1.0002f * bar);
+            if (high > bar) {
+              bar = high;
+              wx = x[h];
+              wq = q[h];
+              wi = v * kPer + h - s.shift;
+            }
           }
         }
       }
     }
-    return Racer{mt, z0 + z1, wx, wi};
+    return Racer{mt, z0 + z1, wx, 2 * wi + (close ? 1 : 0)};
+  }
+
+  // The threads' winners `best` where a thread's lead was not clear: if that thread may hold the
+  // block's winner, the block's elements race again, compared exactly.
+  __device__ __noinline__ u64 settle(u64 best, bool close) const {
+    Sampler me(*this);
+    const u64 top = me.team.block_best(best);
+    const float lead = key_value(static_cast<uint32_t>(top >> 32));
+    const float mine = key_value(static_cast<uint32_t>(best >> 32));
+    if (!__syncthreads_or(close && !(mine * 1.0002f < lead))) return best;
+    Race run;
+    me.s.each([&](int i, float x) {
+      if (x > kNegInf) me.race(run, x, i, me.weight_near(x));
+    });
+    return run.best;
   }
 
   // The row's maximum and sum of weights from the threads'.
@@ -1427,7 +1449,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(const __
     sh.others = -1.0f;
   }
   float mt, zt, wx = 0.0f;
-  int wi = -1;
+  int wi = -2;
   if (open_race) {
     const auto out = Sampler<E>::scan_race(k.s, k.noise, k.c);
     mt = out.top;
@@ -1535,7 +1557,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(const __
         if (x == k.m && e > best) best = e;
       });
     } else if (open_race) {
-      if (wi >= 0) best = k.entry(wx, wi);
+      if (wi >= 0) best = k.entry(wx, wi >> 1);
+      const bool close = (wi & 1) != 0;
+      if (__syncthreads_or(close)) {
+        const Sampler<E> slow = k;
+        best = slow.settle(best, close);
+      }
     } else {
       // the exponent's rounding is far below 1e-4 wherever the weight is above 2^-100
       const float low = k.min_p > 1e-30f ? k.m + (log2f(k.min_p) - 1e-4f) / k.c - fabsf(k.m) * 1e-6f

@@ -31,7 +31,8 @@ def sample(logits: torch.Tensor, noise: torch.Tensor, *, temperature=1.0, top_k=
         return tensors().sample(logits, noise, temperature, top_k, top_p, min_p, out)
     if stream.device != logits.device:
         raise ValueError(f"stream is on {stream.device}, the input on {logits.device}")
-    for x in (logits, noise, temperature, top_k, top_p, min_p, *(out if isinstance(out, tuple) else ())):
+    given = out if isinstance(out, tuple) else ()
+    for x in (logits, noise, temperature, top_k, top_p, min_p, *given):
         if isinstance(x, torch.Tensor) and x.is_cuda:
             x.record_stream(stream)  # used there: keep its memory until the stream has run
     with torch.cuda.stream(stream):

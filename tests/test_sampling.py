@@ -359,3 +359,38 @@ def test_outputs_given_for_another_stream_are_kept_for_it(monkeypatch):
     side.synchronize()
     for t in (x, q, p, *out):
         assert (t.data_ptr(), side) in kept
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [40, 5003, 151936])
+@pytest.mark.parametrize("rows", [64, 600])
+def test_equal_quotients_go_to_the_lowest_index(dtype, vocab, rows):
+    """Constant logits with constant noise of many values, and with noise one step lower at two
+    places (1 / 1.125 and its neighbour's quotient differ in float32)."""
+    x = torch.full((1, vocab), 1.5, device="cuda", dtype=DTYPES[dtype]).expand(rows, vocab)
+    q = torch.linspace(0.01, 7.3, rows, device="cuda")[:, None].expand(rows, vocab).contiguous()
+    for kw in (dict(), dict(temperature=0.7)):
+        tokens, _ = api.sample(x, q, **kw)
+        assert (tokens == 0).all(), kw
+    r = torch.arange(rows, device="cuda")
+    at = (r * 7919 + 3) % (vocab - 1)
+    later = torch.minimum(at + 1 + r % 300, torch.tensor(vocab - 1, device="cuda"))
+    q.fill_(1.125)
+    q[r, at] = q[r, later] = float(np.nextafter(np.float32(1.125), np.float32(0)))
+    tokens, _ = api.sample(x, q)
+    assert torch.equal(tokens.long(), at)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v", [(1, 32003), (40, 5003), (600, 4096)])
+def test_nearly_equal_quotients(dtype, n, v):
+    """Noise that all but follows the weights: without filters the race is decided as it is behind
+    a filter that keeps everything, where each quotient is compared as it is in float32."""
+    x, q = inputs(n, v, dtype, 47, 2.0)
+    w = torch.exp(x.double() - x.double().amax(1, keepdim=True))
+    q = (w * (1 + 1e-6 * torch.randn(n, v, device="cuda", dtype=torch.float64))).float()
+    tokens, _ = api.sample(x, q)
+    kept, _ = api.sample(x, q, min_p=1e-30)
+    assert torch.equal(tokens, kept)
