@@ -287,6 +287,22 @@ struct Sum {
   uint32_t count;
 };
 
+// A sum of many terms in float32: each addition's rounding is kept and taken from the next term.  In
+// a plain sum the roundings of equal terms add up (1e-4 of the sum after 6000 of them).
+struct Long {
+  float sum = 0.0f, over = 0.0f;
+  __device__ __forceinline__ void add(float v) {
+    const float y = v - over, t = sum + y;
+    over = (t - sum) - y;
+    sum = t;
+  }
+  __device__ __forceinline__ void scale(float f) {
+    sum *= f;
+    over *= f;
+  }
+  __device__ __forceinline__ double value() const { return static_cast<double>(sum) - over; }
+};
+
 struct Shared {
   u64 list[kCap];        // the row's candidates, in the first block of the cluster
   union {
@@ -335,8 +351,7 @@ struct Team {
     return blocks > 1 ? cluster.map_shared_rank(p, b) : p;
   }
 
-  __device__ __forceinline__ Sum sum(float mass, uint32_t count) {
-    double m = mass;
+  __device__ __forceinline__ Sum sum(double m, uint32_t count) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       m += __shfl_xor_sync(kAll, m, o);
@@ -381,8 +396,9 @@ struct Team {
     return v;
   }
 
-  __device__ __forceinline__ u64 best(u64 v) {
-    v = block_best(v);
+  __device__ __forceinline__ u64 best(u64 v) { return blocks_best(block_best(v)); }
+  // The same of what each block's threads agree on.
+  __device__ __forceinline__ u64 blocks_best(u64 v) {
     if (blocks == 1) {
       __syncthreads();  // warp_best may be written again
       return v;
@@ -558,32 +574,44 @@ struct Sampler {
   }
 
   // Pass 1 with the filters still to come.  A thread's weights are 2^(x c - ref) with ref the rounded
-  // product of its maximum and c, so one fused multiply-add gives the exponent with one rounding;
-  // join() undoes the difference between ref and the product.  The next group's loads are in
-  // flight while one is summed.  A NaN, which the maxima ignore, makes the sum NaN.
+  // product of one of its values and c, so one fused multiply-add gives the exponent with one
+  // rounding; join() undoes the difference between ref and the product.  ref moves when a value lies
+  // more than kAbove octaves over it, so that a slowly rising row does not rescale at every step.  The
+  // next group's loads are in flight while one is summed.  A NaN, which the maxima ignore, makes the
+  // sum NaN.
+  static constexpr float kAbove = 8.0f;
   struct Running {
     float top = kNegInf, ref = kNegInf;
-    u64 sums = 0;  // two
+    Long sum;
+    // The sum relative to the maximum's own rounded product.
+    __device__ __forceinline__ float settled(float c) const {
+      return top > kNegInf ? (sum.sum - sum.over) * exp2_approx(ref - __fmul_rn(top, c)) : 0.0f;
+    }
   };
   static __device__ __forceinline__ void raise(Running& w, float most, float c) {
-    if (most > w.top) {
+    w.top = fmaxf(w.top, most);
+    if (fmaf(most, c, -w.ref) > kAbove) {
       const float old = w.ref;
-      w.top = most;
       w.ref = __fmul_rn(most, c);
-      const float f = exp2_approx(old - w.ref);
-      float a, b;
-      unpack2(w.sums, a, b);
-      w.sums = pack2(a * f, b * f);
+      w.sum.scale(exp2_approx(old - w.ref));
     }
   }
-  static __device__ __forceinline__ void add(Running& w, const uint4& r, float c) {
+  template <int N>
+  static __device__ __forceinline__ void add(Running& w, const uint4 (&r)[N], float c) {
     const u64 cc = pack2(c, c), rr = pack2(-w.ref, -w.ref);
-    float x[kPer];
-    V::unpack(r, x);
+    u64 sums = 0;  // two
 #pragma unroll
-    for (int q = 0; q < kPer; q += 2) {
-      w.sums = add2(w.sums, exp2_approx2(fma2(pack2(x[q], x[q + 1]), cc, rr)));
+    for (int u = 0; u < N; ++u) {
+      float x[kPer];
+      V::unpack(r[u], x);
+#pragma unroll
+      for (int q = 0; q < kPer; q += 2) {
+        sums = add2(sums, exp2_approx2(fma2(pack2(x[q], x[q + 1]), cc, rr)));
+      }
     }
+    float a, b;
+    unpack2(sums, a, b);
+    w.sum.add(a + b);
   }
 
   struct Stat {
@@ -595,8 +623,8 @@ struct Sampler {
     if (threadIdx.x < 2) {  // the row's first and last vectors
       const int v = threadIdx.x == 0 ? 0 : s.vecs - 1;
       if (v >= s.v0 && v < s.v1 && (threadIdx.x == 0 || v > 0)) {
-        const uint4 r = s.fix(v, __ldg(s.base + v));
-        raise(w, V::max2(r, r), c);
+        const uint4 r[1] = {s.fix(v, __ldg(s.base + v))};
+        raise(w, V::max2(r[0], r[0]), c);
         if (w.top > kNegInf) add(w, r, c);
       }
     }
@@ -630,16 +658,11 @@ struct Sampler {
         const float most = fmaxf(V::max2(now[0], now[1]), V::max2(now[2], now[3]));
         top = fmaxf(top, most);
         raise(w, most, c);
-        if (most > kNegInf) {
-#pragma unroll
-          for (int u = 0; u < kGroup; ++u) add(w, now[u], c);
-        }
+        if (most > kNegInf) add(w, now, c);
       }
       slot[at * kThreads + threadIdx.x] = top;
     }
-    float a, b;
-    unpack2(w.sums, a, b);
-    return Stat{w.top, a + b};
+    return Stat{w.top, w.settled(c)};
   }
 
   // kPer float32 values, read once: 16 or 32 bytes in one load.
@@ -670,7 +693,7 @@ struct Sampler {
 
   // Pass 1 without filters: the race runs along.  A thread keeps the lead among its elements in
   // approximate weights, relative to its maximum, and whether another element came within 1e-4 of
-  // it (the approximation is within 1e-5): then settle() compares exactly.
+  // it (the approximation is within 1e-5): see hides().
   // Bound by memory: 6 bytes an element (16-bit logits) at 4.4 TB/s, 200 rows of 151936 in 41 us.
   struct Racer {
     float top, sum, x;
@@ -678,10 +701,10 @@ struct Sampler {
   };
   static __device__ __noinline__ Racer scan_race(const S s, const float* noise, float c) {
     const bool wide = s.shift == 0 && reinterpret_cast<uintptr_t>(noise) % (4 * kPer) == 0;
-    float mt = kNegInf, wx = kNegInf, wq = 1.0f;  // the maximum; the lead's logit and noise
+    Running z;
+    float wx = kNegInf, wq = 1.0f, bar = 0.0f;  // the lead's logit and noise, 0.9999 of its quotient
     int wi = -1;
     bool close = false;
-    float ref = kNegInf, z0 = 0.0f, z1 = 0.0f, bar = 0.0f;  // bar: 0.9999 of the lead's quotient
     int v = s.v0 + static_cast<int>(threadIdx.x);
     uint4 r = s.raw(v);
     float next[kPer];
@@ -694,25 +717,27 @@ struct Sampler {
       r = s.raw(v + kThreads);
       load_noise(s, noise, v + kThreads, wide, next);
       const float most = V::max2(now, now);
-      if (most > mt) {
-        const float old = ref;
-        mt = most;
-        ref = __fmul_rn(mt, c);
-        const float f = exp2_approx(old - ref);
-        z0 *= f;
-        z1 *= f;
-        // anew: a product for every new maximum would add up its errors
-        bar = 0.9999f * __fdividef(exp2_approx(fmaf(wx, c, -ref)), wq);
-      }
+      const float old = z.ref;
+      raise(z, most, c);
+      if (z.ref != old) bar = 0.9999f * __fdividef(exp2_approx(fmaf(wx, c, -z.ref)), wq);
       if (most > kNegInf) {
-        float x[kPer];
+        float x[kPer], w[kPer];
         V::unpack(now, x);
+        const u64 cc = pack2(c, c), rr = pack2(-z.ref, -z.ref);
+        u64 sums = 0;  // two
+#pragma unroll
+        for (int h = 0; h < kPer; h += 2) {
+          const u64 two = exp2_approx2(fma2(pack2(x[h], x[h + 1]), cc, rr));
+          sums = add2(sums, two);
+          unpack2(two, w[h], w[h + 1]);
+        }
+        float a, b;
+        unpack2(sums, a, b);
+        z.sum.add(a + b);
 #pragma unroll
         for (int h = 0; h < kPer; ++h) {
-          const float w = exp2_approx(fmaf(x[h], c, -ref));
-          if (h & 1) z1 += w; else z0 += w;
-          if (w > bar * q[h] && q[h] >= 0.0f) {
-            const float high = 0.9999f * __fdividef(w, q[h]);
+          if (w[h] > bar * q[h] && q[h] >= 0.0f) {
+            const float high = 0.9999f * __fdividef(w[h], q[h]);
             close = !(high > 1.0002f * bar);
             if (high > bar) {
               bar = high;
@@ -724,22 +749,23 @@ struct Sampler {
         }
       }
     }
-    return Racer{mt, z0 + z1, wx, 2 * wi + (close ? 1 : 0)};
+    return Racer{z.top, z.settled(c), wx, 2 * wi + (close ? 1 : 0)};
   }
 
-  // The threads' winners `best` where a thread's lead was not clear: if that thread may hold the
-  // block's winner, the block's elements race again, compared exactly.
-  __device__ __noinline__ u64 settle(u64 best, bool close) const {
+  // Whether the lead of a thread (its winner `mine`) may hide the winner of the block, whose threads'
+  // winners give `top`.
+  static __device__ __forceinline__ bool hides(u64 mine, u64 top) {
+    return !(key_value(static_cast<uint32_t>(mine >> 32)) * 1.0002f <
+             key_value(static_cast<uint32_t>(top >> 32)));
+  }
+  // Then the block's elements race again, compared exactly.
+  __device__ __noinline__ u64 race_again() const {
     Sampler me(*this);
-    const u64 top = me.team.block_best(best);
-    const float lead = key_value(static_cast<uint32_t>(top >> 32));
-    const float mine = key_value(static_cast<uint32_t>(best >> 32));
-    if (!__syncthreads_or(close && !(mine * 1.0002f < lead))) return best;
     Race run;
     me.s.each([&](int i, float x) {
       if (x > kNegInf) me.race(run, x, i, me.weight_near(x));
     });
-    return run.best;
+    return me.team.block_best(run.best);
   }
 
   // The row's maximum and sum of weights from the threads'.
@@ -1196,7 +1222,7 @@ struct Sampler {
 
   // split()'s pass over the row.
   template <bool FINE>
-  __device__ __forceinline__ void split_vectors(float low, int at, int end, float& za, float& zi,
+  __device__ __forceinline__ void split_vectors(float low, int at, int end, Long& za, Long& zi,
                                                 uint32_t& n, Race& run) {
     // A vector at a time: its noise is loaded at once, and raced where an element may lead.
     const float fine_from = bin_edge(FINE ? fine_of : 0), fine_to = bin_edge(fine_end + 1);
@@ -1219,11 +1245,13 @@ struct Sampler {
       n += __popc(over);
       bool leads = false;
       const float lead = 0.9999f * run.lead;
+      float sum = 0.0f;
 #pragma unroll
       for (int q = 0; q < kPer; ++q) {
-        za += w[q];
+        sum += w[q];
         leads |= ((over >> q) & 1u) && !(w[q] < lead * d[q]);
       }
+      za.add(sum);
       if (leads) {
 #pragma unroll
         for (int q = 0; q < kPer; ++q) {
@@ -1236,7 +1264,7 @@ struct Sampler {
 #pragma unroll
         for (int q = 0; q < kPer; ++q) {
           if ((in >> q) & 1u) {
-            zi += weight_near(x[q]);
+            zi.add(weight_near(x[q]));
             const uint32_t to = atomicAdd(&sh.count, 1u);
             if (to < kCap) put(to, i + q, x[q]);
           }
@@ -1250,7 +1278,7 @@ struct Sampler {
   __device__ __forceinline__ uint32_t split_in(int at, int end, Sum* above, double* inside,
                                                 u64* best) {
     open_list();
-    float za = 0.0f, zi = 0.0f;
+    Long za, zi;
     uint32_t n = 0;
     Race run;
     const float low = bin_floor(fine_of < 0 ? end : fine_end);
@@ -1258,8 +1286,8 @@ struct Sampler {
     else split_vectors<true>(low, at, end, za, zi, n, run);
     float unused;
     const uint32_t listed = close_list(0.0f, &unused);
-    *above = team.sum(za, n);
-    *inside = team.sum(zi, 0).mass;
+    *above = team.sum(za.value(), n);
+    *inside = team.sum(zi.value(), 0).mass;
     *best = team.best(run.best);
     return listed;
   }
@@ -1275,15 +1303,15 @@ struct Sampler {
 
   // Whole passes: the cut in rank order by bisection, then the race over what is above it.
   __device__ __forceinline__ u64 by_passes_in(float* total) {
-    float zt = 0.0f;
+    Long zt;
     uint32_t n = 0;
     s.each([&](int, float x) {
       if (x > kNegInf) {
-        zt += weight(x);
+        zt.add(weight(x));
         ++n;
       }
     });
-    const Sum all = team.sum(zt, n);
+    const Sum all = team.sum(zt.value(), n);
     *total = static_cast<float>(all.mass);
     // Elements above `cut` stay, and the first `ties` of those equal to it.
     float cut = kNegInf;
@@ -1300,15 +1328,15 @@ struct Sampler {
         if (team.sum(0.0f, n).count >= static_cast<uint32_t>(top_k)) lo = mid; else hi = mid;
       }
       cut = short_value(lo);
-      float above = 0.0f;
+      Long above;
       n = 0;
       s.each([&](int, float x) {
         if (x > cut) {
-          above += weight(x);
+          above.add(weight(x));
           ++n;
         }
       });
-      const Sum a = team.sum(above, n);
+      const Sum a = team.sum(above.value(), n);
       ties = static_cast<uint32_t>(top_k) - a.count;
       mass_k = a.mass + static_cast<double>(ties) * weight(cut);
     }
@@ -1320,9 +1348,11 @@ struct Sampler {
       while (hi - lo > 1) {
         const uint32_t mid = lo + (hi - lo) / 2;
         const float v = short_value(mid);
-        float above = 0.0f;
-        s.each([&](int, float x) { above += x > v ? weight(x) : 0.0f; });
-        const Sum a = team.sum(above, 0);
+        Long above;
+        s.each([&](int, float x) {
+          if (x > v) above.add(weight(x));
+        });
+        const Sum a = team.sum(above.value(), 0);
         if (a.mass < target) {
           hi = mid;
           above_hi = a.mass;
@@ -1558,11 +1588,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(const __
       });
     } else if (open_race) {
       if (wi >= 0) best = k.entry(wx, wi >> 1);
-      const bool close = (wi & 1) != 0;
-      if (__syncthreads_or(close)) {
+      const u64 mine = best;
+      best = k.team.block_best(best);
+      if (__syncthreads_or((wi & 1) && Sampler<E>::hides(mine, best))) {
         const Sampler<E> slow = k;
-        best = slow.settle(best, close);
+        best = slow.race_again();
       }
+      best = k.team.blocks_best(best);
     } else {
       // the exponent's rounding is far below 1e-4 wherever the weight is above 2^-100
       const float low = k.min_p > 1e-30f ? k.m + (log2f(k.min_p) - 1e-4f) / k.c - fabsf(k.m) * 1e-6f
@@ -1575,7 +1607,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sample_kernel(const __
       });
       best = run.best;
     }
-    best = k.team.best(best);
+    if (!open_race) best = k.team.best(best);
     passes = open_race && (best >> 32) <= value_key(0.0f);  // every quotient 0 or none
   }
   if (passes) {

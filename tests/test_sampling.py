@@ -394,3 +394,64 @@ def test_nearly_equal_quotients(dtype, n, v):
     tokens, _ = api.sample(x, q)
     kept, _ = api.sample(x, q, min_p=1e-30)
     assert torch.equal(tokens, kept)
+
+
+def long_row(kind, v, dtype):
+    if kind == "flat":  # one token ahead of all others
+        x = torch.full((v,), -0.5, device="cuda")
+        x[0] = 0.0
+    elif kind == "rising":
+        x = torch.linspace(-3.0, 3.0, v, device="cuda")
+    else:  # few values in long runs
+        x = torch.arange(v, device="cuda").div(v / 5.0).floor().mul(-0.375)
+    return x.to(DTYPES[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["flat", "runs", "rising"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,v", [(600, 3000017), (130, 3000017), (2, 2**24 + 5), (1, 2**26)])
+def test_sums_of_long_rows(kind, dtype, n, v):
+    """Sums over millions of equal or slowly changing weights, at many temperatures, in every pass
+    that sums a row: within the bound that holds for every other row."""
+    x = long_row(kind, v, dtype)
+    best = int(x.argmax())
+    t = torch.linspace(0.3, 3.0, n, device="cuda")
+    want = []
+    for r in range(n):
+        z = torch.zeros((), dtype=torch.float64, device="cuda")
+        values, counts = torch.unique(x, return_counts=True) if r == 0 else (values, counts)
+        e = (values.double() - values[-1].double()) / t[r].double()
+        want.append(-torch.log((torch.exp(e) * counts).sum()))
+    want = torch.stack(want)
+    rows, noise = x.expand(n, v), torch.ones((1, v), device="cuda").expand(n, v)
+    settings = [dict(), dict(top_p=0.7), dict(top_k=200)]
+    if n * v < 5e8 and kind != "rising":
+        settings.append(dict(top_k=3000, top_p=0.99))
+    for kw in settings:
+        tokens, logprobs = api.sample(rows, noise, temperature=t, **kw)
+        assert ((x[tokens.long()] - x[best]).abs() <= 1e-5).all(), kw
+        err = (logprobs.double() - want).abs()
+        assert (err <= 4e-6 + 2.0**-21 * want.abs()).all(), (kw, err.max().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,v", [(600, 3000017), (2, 2**24 + 5)])
+@pytest.mark.parametrize("p", [0.3, 0.85])
+def test_nucleus_of_long_flat_rows(n, v, p):
+    """The cut falls among millions of equal tokens: a favoured one 3e-5 of the mass before it is
+    kept, a more favoured one as far behind it is not."""
+    x = long_row("flat", v, "bf16")
+    t = torch.linspace(0.3, 3.0, n, device="cuda")
+    w = torch.exp(-0.5 / t.double())
+    mass = 1.0 + (v - 1) * w
+    p32 = float(np.float32(p))
+    inside = ((p32 * (1 - 3e-5) * mass - 1.0) / w).floor().long()
+    outside = ((p32 * (1 + 3e-5) * mass - 1.0) / w).ceil().long() + 1
+    for r in range(0, n, max(1, n // 12)):
+        noise = torch.ones(v, device="cuda")
+        noise[inside[r]] = 1e-6
+        noise[outside[r]] = 1e-12
+        # the row among as many others as the batch has, so that it gets as many blocks
+        tokens, _ = api.sample(x.expand(n, v), noise.expand(n, v), temperature=float(t[r]), top_p=p)
+        assert (tokens == inside[r]).all(), r
