@@ -321,7 +321,7 @@ struct Shared {
   };
   float2 warp_stat[kWarps];
   float2 block_stat[kMaxCluster];
-  float block_mass[kMaxCluster];
+  u64 block_mass[kMaxCluster];
   uint32_t warp_count[kWarps];
   float warp_mass[kWarps];
   Sum warp_sum[kWarps];
@@ -968,17 +968,18 @@ struct Sampler {
         (static_cast<u64>(~value_key(x)) << 32) | static_cast<uint32_t>(i);
   }
   // Joins the blocks' candidates in the first block's list; their number in the row, and the sum
-  // of all blocks' `part` (a thread's weight of candidates).
-  __device__ __forceinline__ uint32_t close_list(float part, float* mass) {
+  // of all blocks' `part` (a thread's weight of candidates, in units of 2^-32: which thread took which
+  // candidate differs from run to run, and whole numbers add up to the same all the same).
+  __device__ __forceinline__ uint32_t close_list(u64 part, float* mass) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(kAll, part, o);
-    if ((threadIdx.x & 31) == 0) sh.warp_mass[threadIdx.x >> 5] = part;
+    if ((threadIdx.x & 31) == 0) sh.warp_best[threadIdx.x >> 5] = part;
     __syncthreads();
-    float sum = 0.0f;
+    u64 sum = 0;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) sum += sh.warp_mass[i];
+    for (int i = 0; i < kWarps; ++i) sum += sh.warp_best[i];
     const uint32_t n = sh.count;
-    *mass = sum;
+    *mass = static_cast<float>(sum) * 0x1p-32f;
     if (team.blocks == 1) return n;
     if (threadIdx.x == 0) sh.base = atomicAdd(team.of(&sh.total, 0), n);
     if (threadIdx.x < static_cast<unsigned>(team.blocks)) {
@@ -991,20 +992,20 @@ struct Sampler {
       to[base + i] = sh.sorted[i];
     }
     team.cluster.sync();
-    sum = 0.0f;
+    sum = 0;
     for (int b = 0; b < team.blocks; ++b) sum += sh.block_mass[b];
-    *mass = sum;
+    *mass = static_cast<float>(sum) * 0x1p-32f;
     return *team.of(&sh.total, 0);
   }
 
   // The elements of the bins up to `last`, from the groups that reach it.
   __device__ __forceinline__ uint32_t gather(int last, float* mass) {
-    float part = 0.0f;
+    u64 part = 0;
     const float low = bin_floor(last);
     each_hot(low, [&](int i, float x, bool in) {
       in = in && x > kNegInf && bin(x) <= last;
       push(i, x, in);
-      if (in) part += exp2_approx((x - m) * c);
+      if (in) part += __float2ull_rn(exp2_approx((x - m) * c) * 0x1p32f);
     });
     return close_list(part, mass);
   }
@@ -1285,7 +1286,7 @@ struct Sampler {
     if (fine_of < 0) split_vectors<false>(low, at, end, za, zi, n, run);
     else split_vectors<true>(low, at, end, za, zi, n, run);
     float unused;
-    const uint32_t listed = close_list(0.0f, &unused);
+    const uint32_t listed = close_list(0, &unused);
     *above = team.sum(za.value(), n);
     *inside = team.sum(zi.value(), 0).mass;
     *best = team.best(run.best);

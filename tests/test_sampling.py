@@ -455,3 +455,17 @@ def test_nucleus_of_long_flat_rows(n, v, p):
         # the row among as many others as the batch has, so that it gets as many blocks
         tokens, _ = api.sample(x.expand(n, v), noise.expand(n, v), temperature=float(t[r]), top_p=p)
         assert (tokens == inside[r]).all(), r
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+@pytest.mark.parametrize("n", [7, 300])
+def test_same_nucleus_call_gives_the_same_bits(dtype, n):
+    """Nuclei of some hundred to some thousand tokens, about the size at which the list ends."""
+    x, q = inputs(n, 50001, dtype, 53, 2.0)
+    t = torch.linspace(0.6, 1.6, n, device="cuda")
+    for p in (0.2, 0.5, 0.8):
+        a = api.sample(x, q, temperature=t, top_p=p)
+        for _ in range(5):
+            b = api.sample(x, q, temperature=t, top_p=p)
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
