@@ -241,11 +241,9 @@ struct Slice {
     }
     return r;
   }
-  __device__ __forceinline__ uint4 load(int v) const { return V::clean(fix(v, raw(v))); }
 
-  // f(index, value) for every element of the vectors of the slice whose maximum passes; four
-  // vectors in flight.
-  // f(index, values) for the vectors that `pass`; places outside the row hold -inf.
+  // f(index, values) for the vectors of the slice whose maximum passes, four in flight; places
+  // outside the row hold -inf.
   template <class P, class F>
   __device__ __forceinline__ void each_vector(P pass, F f) const {
     for (int first = v0 + static_cast<int>(threadIdx.x); first < v1; first += kGroup * kThreads) {
@@ -267,16 +265,13 @@ struct Slice {
       }
     }
   }
-  template <class P, class F>
-  __device__ __forceinline__ void each(P pass, F f) const {
-    each_vector(pass, [&](int i, const float (&x)[kPer]) {
+  // f(index, value) for every element.
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    each_vector([](float) { return true; }, [&](int i, const float (&x)[kPer]) {
 #pragma unroll
       for (int q = 0; q < kPer; ++q) f(i + q, x[q]);
     });
-  }
-  template <class F>
-  __device__ __forceinline__ void each(F f) const {
-    each([](float) { return true; }, f);
   }
 };
 
@@ -481,7 +476,7 @@ struct Sampler {
                : kBins;
   }
   // Bins [fine_of, fine_end] that hold too much are binned again, linearly in the value from their
-  // upper edge; elements of the bins before them are in fine bin -1, those after them in kBins.
+  // upper edge.
   int fine_of = -1, fine_end = -1;
   float fine_top = 0.0f, fine_scale = 0.0f;
   __device__ __forceinline__ void refine(int b, int end) {
@@ -489,13 +484,6 @@ struct Sampler {
     fine_end = end;
     fine_top = m - bin_start(b) * (1.0f / 64.0f) / c;
     fine_scale = static_cast<float>(kBins) * 64.0f * c / (bin_start(end + 1) - bin_start(b));
-  }
-  __device__ __forceinline__ int fine_bin(float x) const {
-    const int b = bin(x);
-    if (fine_of < 0 || b >= kBins) return b;
-    if (b < fine_of) return -1;
-    if (b > fine_end) return kBins;
-    return fine_place(x);
   }
   __device__ __forceinline__ int fine_place(float x) const {  // of an element of the bins binned again
     return min(max(static_cast<int>((fine_top - x) * fine_scale), 0), kBins - 1);
@@ -1040,10 +1028,9 @@ struct Sampler {
   }
   // One element's count and weight to its bin; `units` of them are the weight at the bin's start.
   __device__ __forceinline__ void weigh_one(float x, float units) {
-    const int b = fine_bin(x);
-    if (b < 0 || b >= kBins) return;
-    const float past = x == m ? 0.0f : fmaf(m - x, c * 64.0f, 256.0f) -
-                                           (bin_start(fine_of < 0 ? b : fine_of) + 256.0f);
+    const int b = bin(x);
+    if (b >= kBins) return;
+    const float past = x == m ? 0.0f : fmaf(m - x, c * 64.0f, 256.0f) - (bin_start(b) + 256.0f);
     atomicAdd(&sh.bins[b], 1u);
     atomicAdd(&sh.weights[b],
               static_cast<uint32_t>(exp2_approx(past * (-1.0f / 64.0f)) * units + 0.5f));
