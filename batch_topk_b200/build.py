@@ -52,6 +52,14 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(p) <= t for p in [*SOURCES, *HEADERS])
 
 
+def torch_dir() -> str | None:
+    """Where torch is installed, without importing it."""
+    from importlib.util import find_spec
+
+    spec = find_spec("torch")
+    return os.path.dirname(spec.origin) if spec else None
+
+
 def tensors_up_to_date() -> bool:
     if not os.path.exists(TENSORS):
         return False
@@ -68,23 +76,23 @@ def _run(cmd: list[str], verbose: bool = False) -> None:
 
 
 def build_tensors(force: bool = False) -> str:
-    """The Python module; LIB has to be there (it is linked, and found beside the module)."""
+    """The Python module, which needs torch; LIB has to be there (it is linked, and found beside the
+    module)."""
     if not force and tensors_up_to_date():
         return TENSORS
     import sysconfig
-    from importlib.util import find_spec
 
-    torch_dir = os.path.dirname(find_spec("torch").origin)
+    torch = torch_dir()
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     tmp = TENSORS + ".tmp"
     # the g++ that nvcc compiles host code with: another one may bring its own C++ library
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
           "-D_GLIBCXX_USE_CXX11_ABI=1",
-          "-I" + os.path.join(torch_dir, "include"),
-          "-I" + os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+          "-I" + os.path.join(torch, "include"),
+          "-I" + os.path.join(torch, "include", "torch", "csrc", "api", "include"),
           "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda, "include"),
           TENSORS_SRC, "-o", tmp,
-          "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+          "-L" + os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
           "-ltorch_python", "-L" + LIB_DIR, "-lbatch_topk_b200", "-Wl,-rpath,$ORIGIN/lib"])
     os.replace(tmp, TENSORS)
     return TENSORS
@@ -99,7 +107,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
             cmd.insert(1, "-Xptxas=-v")
         _run(cmd, verbose)
         os.replace(tmp, LIB)
-    build_tensors(force)
+    if torch_dir():  # C callers of the library need no torch
+        build_tensors(force)
     return LIB
 
 
