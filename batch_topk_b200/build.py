@@ -30,6 +30,7 @@ LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libbatch_topk_b200.so")
 TENSORS_SRC = os.path.join(HERE, "csrc", "tensors.cpp")  # needs torch's headers
 TENSORS = os.path.join(HERE, "_tensors.so")
+TENSORS_STAMP = os.path.join(HERE, "_build", "torch")  # the torch that TENSORS was built for
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -60,9 +61,17 @@ def torch_dir() -> str | None:
     return os.path.dirname(spec.origin) if spec else None
 
 
+def torch_version() -> str:
+    with open(os.path.join(torch_dir(), "version.py")) as f:
+        return f.read()
+
+
 def tensors_up_to_date() -> bool:
-    if not os.path.exists(TENSORS):
+    if not os.path.exists(TENSORS) or not os.path.exists(TENSORS_STAMP):
         return False
+    with open(TENSORS_STAMP) as f:
+        if f.read() != torch_version():
+            return False
     t = os.path.getmtime(TENSORS)
     return all(os.path.getmtime(p) <= t for p in [TENSORS_SRC, *HEADERS])
 
@@ -94,6 +103,9 @@ def build_tensors(force: bool = False) -> str:
           TENSORS_SRC, "-o", tmp,
           "-L" + os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
           "-ltorch_python", "-L" + LIB_DIR, "-lbatch_topk_b200", "-Wl,-rpath,$ORIGIN/lib"])
+    os.makedirs(os.path.dirname(TENSORS_STAMP), exist_ok=True)
+    with open(TENSORS_STAMP, "w") as f:
+        f.write(torch_version())
     os.replace(tmp, TENSORS)
     return TENSORS
 

@@ -25,6 +25,7 @@ def compiled(monkeypatch, tmp_path):
     monkeypatch.setattr(build, "LIB_DIR", str(tmp_path / "lib"))
     monkeypatch.setattr(build, "LIB", str(tmp_path / "lib" / "lib.so"))
     monkeypatch.setattr(build, "TENSORS", str(tmp_path / "_tensors.so"))
+    monkeypatch.setattr(build, "TENSORS_STAMP", str(tmp_path / "_build" / "torch"))
     return started
 
 
@@ -38,3 +39,21 @@ def test_library_builds_where_torch_is_not_installed(monkeypatch, compiled):
     torch_at(monkeypatch, None)
     assert build.build() == build.LIB and os.path.exists(build.LIB)
     assert compiled == ["nvcc"] and not os.path.exists(build.TENSORS)
+
+
+def test_module_is_built_again_for_another_torch(monkeypatch, compiled, tmp_path):
+    places = []
+    for version in ("1", "2"):
+        place = tmp_path / version
+        place.mkdir()
+        (place / "version.py").write_text(f"__version__ = {version!r}\n")
+        os.utime(place / "version.py", (0, 0))  # as a wheel may install it
+        places.append(place)
+    torch_at(monkeypatch, places[0])
+    build.build()
+    build.build()
+    assert compiled == ["nvcc", "g++"]
+    torch_at(monkeypatch, places[1])
+    build.build()
+    build.build()
+    assert compiled == ["nvcc", "g++", "g++"]
