@@ -741,10 +741,11 @@ struct Sampler {
   }
 
   // Whether the lead of a thread (its winner `mine`) may hide the winner of the block, whose threads'
-  // winners give `top`.
+  // winners give `top`.  Quotients of 0 hide nothing: should the row have no other, whole passes
+  // decide.
   static __device__ __forceinline__ bool hides(u64 mine, u64 top) {
-    return !(key_value(static_cast<uint32_t>(mine >> 32)) * 1.0002f <
-             key_value(static_cast<uint32_t>(top >> 32)));
+    const float lead = key_value(static_cast<uint32_t>(top >> 32));
+    return lead > 0.0f && !(key_value(static_cast<uint32_t>(mine >> 32)) * 1.0002f < lead);
   }
   // Then the block's elements race again, compared exactly.
   __device__ __noinline__ u64 race_again() const {
