@@ -686,3 +686,65 @@ def test_arguments_that_cannot_be_read():
         api.route(x, 2, renormalize=Unclear())
     with pytest.raises(ValueError):
         api.route(x, 2, score="\ud800")
+
+
+@pytest.mark.gpu
+def test_whole_layer_in_a_graph():
+    """A training step of route, order, dispatch and combine, captured and replayed on new inputs."""
+    x = rand(517, 256, seed=51, dtype="bf16").requires_grad_()
+    logits = rand(517, 64, seed=52).requires_grad_()
+    g = rand(517, 256, seed=53, dtype="bf16")
+
+    def step():
+        weights, experts = api.route(logits, 9, score="sigmoid")
+        plan = api.expert_order(experts, 64)
+        y = api.combine(api.dispatch(x, plan), plan, weights)
+        return (y, *torch.autograd.grad(y, (x, logits), g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (54, 55):
+        with torch.no_grad():
+            x.copy_(rand(517, 256, seed=seed, dtype="bf16"))
+            logits.copy_(rand(517, 64, seed=seed + 10))
+        graph.replay()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_calls_from_threads():
+    """Each thread on a stream of its own, with orders of one and of several blocks."""
+    import threading
+
+    def layer(seed, tokens):
+        weights, experts = api.route(rand(tokens, 64, seed=seed), 8)
+        plan = api.expert_order(experts, 64)
+        y = api.combine(api.dispatch(rand(tokens, 64, seed=seed + 1), plan), plan, weights)
+        return (*plan, y)
+
+    sizes = [(i, (300, 4001)[i % 2]) for i in range(4)]
+    want = [layer(*s) for s in sizes]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = layer(*sizes[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
