@@ -8,8 +8,9 @@ re-exports it).
                                                      # plan.offsets[e]:plan.offsets[e + 1] for e
     y = combine(rows, plan, weights)                 # [tokens, width]
 
-``route``, ``dispatch`` and ``combine`` have (first-order) gradients.  Semantics, ties and empty slots are those
-of the ``bt_`` entry points in include/batch_topk_b200.h.  No reference counterpart: the reference
+``route``, ``dispatch`` and ``combine`` have first-order gradients; forward-mode derivatives and
+differentiating a gradient again raise a RuntimeError.  Semantics, ties and empty slots are those of
+the ``bt_`` entry points in include/batch_topk_b200.h.  No reference counterpart: the reference
 ends with the top k (include/batch_topk.cuh:10-19).
 """
 from __future__ import annotations
@@ -26,7 +27,10 @@ class ExpertOrder(NamedTuple):
 
     offsets [experts + 1]: expert e's assignments are order[offsets[e]:offsets[e + 1]];
     order [tokens * k]: which assignment (token * k + slot) stands at a place, -1 past the last;
-    position [tokens, k]: the place of an assignment, -1 where its expert is none."""
+    position [tokens, k]: the place of an assignment, -1 where its expert is none.
+
+    order and position are each other's inverse, which the gradients of dispatch and combine rely
+    on."""
 
     offsets: torch.Tensor
     order: torch.Tensor

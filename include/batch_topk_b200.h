@@ -265,9 +265,9 @@ int bt_combine(const void* d_rows, int elem, int tokens, int k, int width, const
                const float* d_weights, void* d_y, void* stream);
 
 /* bt_combine's gradients: d_rows_grad[p] = weight * grad of the token that row p belongs to (rows
- * from *d_live on, which belong to none, are zero; d_live is d_offsets + experts), and
- * d_weights_grad[t, j] = <grad[t], d_rows[d_position[t, j]]>.  Either output may be NULL;
- * d_rows is read for d_weights_grad only. */
+ * from *d_live on, which belong to none, are zero; d_live is d_offsets + experts; d_position
+ * names every row before it), and d_weights_grad[t, j] = <grad[t], d_rows[d_position[t, j]]>, 0 where
+ * the position is -1.  Either output may be NULL; d_rows is read for d_weights_grad only. */
 int bt_combine_backward(const void* d_rows, const void* d_grad, int elem, int tokens, int k,
                         int width, long long grad_stride, const int* d_position,
                         const int* d_live, const float* d_weights, void* d_rows_grad,
